@@ -31,6 +31,14 @@ __all__ = [
     "gemmrc_host",
     "gemmrc_host_rows",
     "gemmrc_allgather",
+    "gated_gemmrc",
+    "gated_gemmrc_backward",
+    "gemmrc_backward",
+    "mxfp4_empty",
+    "mxfp4_tile_scales",
+    "mxfp4_quantize",
+    "mxfp4_dequantize",
+    "mxfp4_gemmrc",
     "splitk_describe",
     "release_workspaces",
     "BeamError",
@@ -101,6 +109,14 @@ def _load():
     L.beam_gemmrc_fp16_host_rows.argtypes = [vp, vp, vp, i, i, i]
     L.beam_gemmrc_silu.argtypes = [vp, vp, vp, i, i, i, vp, vp, ctypes.c_longlong, vp]
     L.beam_gemmrc_fp16_allgather.argtypes = [vp, vp, ctypes.POINTER(vp), i, i, i, i, i, ctypes.POINTER(beam_gemm_cfg), vp]
+    L.beam_gated_gemmrc.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, i, vp]
+    L.beam_gated_gemmrc_backward_workspace_bytes.restype = sz
+    L.beam_gated_gemmrc_backward_workspace_bytes.argtypes = [i, i, i]
+    L.beam_gated_gemmrc_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, vp, sz, vp]
+    L.beam_gemmrc_backward.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp]
+    L.beam_mxfp4_quantize.argtypes = [vp, vp, vp, i, i, i, vp]
+    L.beam_mxfp4_dequantize.argtypes = [vp, vp, vp, i, i, i, vp]
+    L.beam_mxfp4_gemmrc.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp]
     _lib = L
     return L
 
@@ -353,6 +369,189 @@ def gemmrc_allgather(a_local, b, gathered_ptrs, rank, n, tile_n=0, cta_pair=0, s
                                           cfg, _stream(a_local))
     if st != BEAM_OK:
         _raise(st, "beam_gemmrc_fp16_allgather")
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+_HALF_TYPES = (torch.float16, torch.bfloat16)
+
+
+def _check_matrix(name, t, shape, dtype, device):
+    """A contiguous CUDA tensor of this shape, type and device; shape or device None: any of two dimensions, any CUDA device;
+    dtype may be a tuple of choices."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor" % name)
+    if t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if not t.is_cuda:
+        raise ValueError("%s must be a CUDA tensor (there is no CPU path)" % name)
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    if t.dim() != (2 if shape is None else len(shape)) or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError("%s must be %s, got %s" % (name, "2-D" if shape is None else tuple(shape), tuple(t.shape)))
+    if device is not None and t.device != device:
+        raise ValueError("%s must be on %s, like the other tensors" % (name, device))
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError("activation must be one of %s, got %r" % (", ".join(ACTIVATIONS), name))
+    return ACTIVATIONS[name]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _half_flags(t):
+    return 2 if t.dtype == torch.bfloat16 else 0
+
+
+def _call(fn_name, device, *args):
+    """Calls a C entry with `device` current, on torch's current stream of that device (its last argument)."""
+    L = _load()
+    with torch.cuda.device(device):
+        st = getattr(L, fn_name)(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    if st != BEAM_OK:
+        _raise(st, fn_name)
+
+
+def gated_gemmrc(a, b_gate, b_up, c, activation="silu", gate=None, up=None):
+    """c[M,F] = act(a @ b_gate.T) * (a @ b_up.T) in one kernel: the gated half of a feed-forward block.
+
+    a [M,K], b_gate and b_up [F,K], c [M,F], all float16 or all bfloat16, K and F multiples of 8.  activation: "silu", "gelu"
+    (the erf form), "gelu_tanh" or "relu".  The products are accumulated and combined in fp32 and c is rounded once.
+    gate and up, given together, are [M,F] outputs that keep the two products for gated_gemmrc_backward."""
+    act = _activation(activation)
+    _check_matrix("a", a, None, _HALF_TYPES, None)
+    m, k = a.shape
+    _check_matrix("b_gate", b_gate, None, a.dtype, a.device)
+    f = b_gate.shape[0]
+    _check_matrix("b_gate", b_gate, (f, k), a.dtype, a.device)
+    _check_matrix("b_up", b_up, (f, k), a.dtype, a.device)
+    _check_matrix("c", c, (m, f), a.dtype, a.device)
+    if (gate is None) != (up is None):
+        raise ValueError("gate and up must be given together")
+    if gate is not None:
+        _check_matrix("gate", gate, (m, f), a.dtype, a.device)
+        _check_matrix("up", up, (m, f), a.dtype, a.device)
+    _call("beam_gated_gemmrc", a.device, a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(), c.data_ptr(), _ptr(gate),
+          _ptr(up), m, f, k, act, _half_flags(a))
+
+
+def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, db_up=None, activation="silu"):
+    """Gradients of gated_gemmrc: with dg = dc * up * act'(gate) and du = dc * act(gate),
+
+        da = dg @ b_gate + du @ b_up,   db_gate = dg.T @ a,   db_up = du.T @ a.
+
+    dc, gate and up are [M,F]; gate and up are what the forward call kept.  The gradients wanted are given as tensors
+    (at least one) and overwritten.  dg and du are rounded to the operands' type between the two steps; they are
+    held in scratch of 4 M F bytes from torch's allocator."""
+    act = _activation(activation)
+    _check_matrix("a", a, None, _HALF_TYPES, None)
+    m, k = a.shape
+    _check_matrix("b_gate", b_gate, None, a.dtype, a.device)
+    f = b_gate.shape[0]
+    wanted = [("b_gate", b_gate, (f, k)), ("b_up", b_up, (f, k)), ("dc", dc, (m, f)), ("gate", gate, (m, f)),
+              ("up", up, (m, f))]
+    wanted += [(name, t, shape) for name, t, shape in (("da", da, (m, k)), ("db_gate", db_gate, (f, k)),
+                                                       ("db_up", db_up, (f, k))) if t is not None]
+    if len(wanted) == 5:
+        raise ValueError("at least one of da, db_gate and db_up must be given")
+    for name, t, shape in wanted:
+        _check_matrix(name, t, shape, a.dtype, a.device)
+    nbytes = _load().beam_gated_gemmrc_backward_workspace_bytes(m, f, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+    _call("beam_gated_gemmrc_backward", a.device, dc.data_ptr(), a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(),
+          gate.data_ptr(), up.data_ptr(), _ptr(da), _ptr(db_gate), _ptr(db_up), m, f, k, act, _half_flags(a),
+          ws.data_ptr(), nbytes)
+
+
+def gemmrc_backward(dc, a, b, da=None, db=None):
+    """Gradients of c = a @ b.T: da[M,K] = dc[M,N] @ b[N,K] and db[N,K] = dc.T @ a[M,K], in one launch.  All tensors
+    float16 or all bfloat16; the gradients wanted are given (at least one) and overwritten; N and K multiples of 8."""
+    _check_matrix("a", a, None, _HALF_TYPES, None)
+    m, k = a.shape
+    _check_matrix("b", b, None, a.dtype, a.device)
+    n = b.shape[0]
+    _check_matrix("b", b, (n, k), a.dtype, a.device)
+    _check_matrix("dc", dc, (m, n), a.dtype, a.device)
+    if da is None and db is None:
+        raise ValueError("at least one of da and db must be given")
+    if da is not None:
+        _check_matrix("da", da, (m, k), a.dtype, a.device)
+    if db is not None:
+        _check_matrix("db", db, (n, k), a.dtype, a.device)
+    _call("beam_gemmrc_backward", a.device, dc.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(da), _ptr(db), m, n, k,
+          _half_flags(a))
+
+
+def _mxfp4_scales_shape(rows, k):
+    return (-(-rows // 128), -(-k // 128), 512)
+
+
+def mxfp4_empty(rows, k, device=None):
+    """Uninitialised (q, scales) of a [rows, k] MXFP4 matrix, k a multiple of 32: q uint8 [rows, k / 2], two codes per byte;
+    scales uint8 [ceil(rows / 128), ceil(k / 128), 512], see mxfp4_tile_scales."""
+    rows, k = int(rows), int(k)
+    if rows <= 0 or k <= 0 or k % 32:
+        raise ValueError("rows must be positive and k a positive multiple of 32, got %d, %d" % (rows, k))
+    device = torch.device("cuda") if device is None else device
+    return (torch.empty(rows, k // 2, dtype=torch.uint8, device=device),
+            torch.empty(_mxfp4_scales_shape(rows, k), dtype=torch.uint8, device=device))
+
+
+def mxfp4_tile_scales(scales):
+    """Row-major scale bytes [rows, k / 32], as files hold them, in the layout of the kernels: blocks of 128 rows x 4 scales,
+    row r and scale c of a block at byte (r % 32) * 16 + (r // 32) * 4 + c, zeros outside the matrix.  Done once per weight."""
+    if not (isinstance(scales, torch.Tensor) and scales.dtype == torch.uint8 and scales.dim() == 2):
+        raise TypeError("scales must be a 2-D uint8 tensor")
+    rows, cols = scales.shape
+    rb, cb = -(-rows // 128), -(-cols // 4)
+    whole = torch.zeros(rb * 128, cb * 4, dtype=torch.uint8, device=scales.device)
+    whole[:rows, :cols] = scales
+    return whole.view(rb, 4, 32, cb, 4).permute(0, 3, 2, 1, 4).reshape(rb, cb, 512).contiguous()
+
+
+def _check_mxfp4(name, q, scales, device=None):
+    """(rows, k) of a quantised matrix."""
+    _check_matrix(name, q, None, torch.uint8, device)
+    rows, k = q.shape[0], q.shape[1] * 2
+    if k % 32:
+        raise ValueError("%s must hold a multiple of 32 elements per row, got %d" % (name, k))
+    _check_matrix(name + "'s scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, q.device)
+    return rows, k
+
+
+def mxfp4_quantize(x, q, scales):
+    """x [rows, k] (float16 or bfloat16) to MXFP4: q and scales as from mxfp4_empty(rows, k).
+
+    The scale of 32 elements is 2 to the power floor(log2(max |x|)) - 2; elements are rounded to the nearest of 0, 0.5, 1, 1.5,
+    2, 3, 4, 6 times it, ties to even codes, and magnitudes above 6 become 6.  A block with an infinity or a NaN becomes NaN."""
+    _check_matrix("x", x, None, _HALF_TYPES, None)
+    rows, k = _check_mxfp4("q", q, scales, x.device)
+    _check_matrix("x", x, (rows, k), _HALF_TYPES, None)
+    _call("beam_mxfp4_quantize", x.device, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, k, _half_flags(x))
+
+
+def mxfp4_dequantize(q, scales, x):
+    """The values of an MXFP4 matrix in x [rows, k], float16, bfloat16 or float32 (exact in the latter two)."""
+    rows, k = _check_mxfp4("q", q, scales)
+    _check_matrix("x", x, (rows, k), _HALF_TYPES + (torch.float32,), q.device)
+    kind = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}[x.dtype]
+    _call("beam_mxfp4_dequantize", q.device, q.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, k, kind)
+
+
+def mxfp4_gemmrc(a, a_scales, b, b_scales, c):
+    """c[M,N] = a @ b.T of two MXFP4 matrices a [M,K] and b [N,K] on the 4-bit tensor cores: fp32 accumulation, c (float16 or
+    bfloat16) rounded once.  N a multiple of 8, K of 32.  Scale bytes outside the matrices must be 0, as mxfp4_quantize
+    and mxfp4_tile_scales leave them."""
+    m, k = _check_mxfp4("a", a, a_scales)
+    n, kb = _check_mxfp4("b", b, b_scales, a.device)
+    if k != kb:
+        raise ValueError("a holds %d elements per row but b %d" % (k, kb))
+    _check_matrix("c", c, (m, n), _HALF_TYPES, a.device)
+    _call("beam_mxfp4_gemmrc", a.device, a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(),
+          c.data_ptr(), m, n, k, _half_flags(c))
 
 
 def gemmrc_host(a, b, c):

@@ -2,9 +2,11 @@
 // Nothing here touches torch; pointers and sizes only.
 #include <cstring>
 
+#include "feedforward_launch.h"
 #include "gemmrc_launch.h"
 #include "host_entry.h"
 #include "layernorm_launch.h"
+#include "mxfp4_launch.h"
 #include "splitk_launch.h"
 
 using namespace beam;
@@ -180,6 +182,52 @@ int beam_gemmrc_layernorm(const void* X, const void* W, void* out, const void* g
 int beam_gemmrc_silu(const void* A, const void* B, void* C, int m, int n, int k, const void* x, void* y,
                      long long count, void* stream) {
   return launch_gemm_silu(A, B, C, m, n, k, x, y, count, static_cast<cudaStream_t>(stream));
+}
+
+int beam_gated_gemmrc(const void* A, const void* B_gate, const void* B_up, void* C, void* gate, void* up, int m, int f,
+                      int k, int activation, int flags, void* stream) {
+  if (flags & ~BEAM_FLAG_BF16) return BEAM_ERR_INVALID_ARG;
+  return launch_gated(A, B_gate, B_up, C, gate, up, m, f, k, activation, flags & BEAM_FLAG_BF16 ? 1 : 0,
+                      static_cast<cudaStream_t>(stream));
+}
+
+size_t beam_gated_gemmrc_backward_workspace_bytes(int m, int f, int k) {
+  return k > 0 ? gated_backward_workspace_bytes(m, f) : 0;
+}
+
+int beam_gated_gemmrc_backward(const void* dC, const void* A, const void* B_gate, const void* B_up, const void* gate,
+                               const void* up, void* dA, void* dB_gate, void* dB_up, int m, int f, int k, int activation,
+                               int flags, void* workspace, size_t workspace_bytes, void* stream) {
+  if (flags & ~BEAM_FLAG_BF16) return BEAM_ERR_INVALID_ARG;
+  return launch_gated_backward(dC, A, B_gate, B_up, gate, up, dA, dB_gate, dB_up, m, f, k, activation,
+                               flags & BEAM_FLAG_BF16 ? 1 : 0, workspace, workspace_bytes,
+                               static_cast<cudaStream_t>(stream));
+}
+
+int beam_gemmrc_backward(const void* dC, const void* A, const void* B, void* dA, void* dB, int m, int n, int k, int flags,
+                         void* stream) {
+  if (flags & ~BEAM_FLAG_BF16) return BEAM_ERR_INVALID_ARG;
+  return launch_gemmrc_backward(dC, A, B, dA, dB, m, n, k, flags & BEAM_FLAG_BF16 ? 1 : 0,
+                                static_cast<cudaStream_t>(stream));
+}
+
+size_t beam_mxfp4_scales_bytes(int rows, int k) { return mxfp4_scales_bytes(rows, k); }
+
+int beam_mxfp4_quantize(const void* x, void* q, void* scales, int rows, int k, int flags, void* stream) {
+  if (flags & ~BEAM_FLAG_BF16) return BEAM_ERR_INVALID_ARG;
+  return launch_mxfp4_quantize(x, q, scales, rows, k, flags & BEAM_FLAG_BF16 ? 1 : 0, static_cast<cudaStream_t>(stream));
+}
+
+int beam_mxfp4_dequantize(const void* q, const void* scales, void* x, int rows, int k, int type, void* stream) {
+  if (type < BEAM_TYPE_FP16 || type > BEAM_TYPE_FP32) return BEAM_ERR_INVALID_ARG;
+  return launch_mxfp4_dequantize(q, scales, x, rows, k, type, static_cast<cudaStream_t>(stream));
+}
+
+int beam_mxfp4_gemmrc(const void* A, const void* a_scales, const void* B, const void* b_scales, void* C, int m, int n,
+                      int k, int flags, void* stream) {
+  if (flags & ~BEAM_FLAG_BF16) return BEAM_ERR_INVALID_ARG;
+  return launch_mxfp4_gemmrc(A, a_scales, B, b_scales, C, m, n, k, flags & BEAM_FLAG_BF16 ? 1 : 0,
+                             static_cast<cudaStream_t>(stream));
 }
 
 int beam_gemmrc_fp16_host(const void* A_host, const void* B_host, void* C_host, int m, int n, int k) {

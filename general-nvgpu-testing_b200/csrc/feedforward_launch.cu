@@ -1,0 +1,261 @@
+// Host launchers of the gated product and of the gradients of rc products.
+#include "feedforward_launch.h"
+
+#include "gated_umma.cuh"
+#include "grad_umma.cuh"
+#include "launch_common.h"
+
+namespace beam {
+
+namespace {
+
+struct GatedPlan {
+  int ctas;   // per tile
+  int width;  // columns of F per tile
+};
+
+// Up to 128 rows one CTA's tile holds them all and the weights are read once whatever the width, so the width only
+// deals out F: the smallest multiple of 8 with which the columns take as few waves of all SMs as 128-wide tiles would.
+// Above, pairs work on 256 rows; 128 columns per tile amortise A best, and a narrower tile is taken only where it saves
+// more in the last wave than it loses in the others.
+GatedPlan gated_plan(int m, int f, int sm_count, int pairs) {
+  GatedPlan plan;
+  if (m <= 128) {
+    plan.ctas = 1;
+    const int waves = ceil_div(f, 128 * sm_count);
+    plan.width = (ceil_div(f, waves * sm_count) + 7) / 8 * 8;
+    return plan;
+  }
+  plan.ctas = 2;
+  plan.width = 128;
+  double best = 0;
+  for (int width = 128; width >= 32; width -= 32) {
+    const long long tiles = static_cast<long long>(ceil_div(m, 256)) * ceil_div(f, width);
+    const double cost = static_cast<double>((tiles + pairs - 1) / pairs) * (width > 64 ? width : 64);
+    if (best == 0 || cost < best) {
+      best = cost;
+      plan.width = width;
+    }
+  }
+  return plan;
+}
+
+template <int kCta>
+int launch_gated_instance(DeviceCtx* ctx, const GatedPlan& plan, int resident, const void* A, const void* Bg,
+                          const void* Bu, void* C, void* G, void* U, int m, int f, int k, int activation, int bf16,
+                          cudaStream_t stream) {
+  using S = GatedShape<kCta>;
+  GatedParams p = {};
+  p.m = m;
+  p.f = f;
+  p.k = k;
+  p.width = plan.width;
+  p.act = activation;
+  p.bf16 = bf16;
+  p.out[0] = C;
+  p.out[1] = G;
+  p.out[2] = U;
+  p.status = ctx->status_word;
+  p.a_rows = kCta == 2 ? S::kBM : (m + 7) / 8 * 8;
+  p.stage_bytes = S::kABytes + p.width * 128 * (kCta == 2 ? 1 : 2);
+  p.stages = S::kRingBytes / p.stage_bytes;
+  if (p.stages > S::kMaxStages) p.stages = S::kMaxStages;
+  p.m_tiles = ceil_div(m, S::kBM * kCta);
+  p.n_tiles = ceil_div(f, p.width);
+  p.group_m = 8;
+  int st = encode_tmap_2d(&p.tm_a, A, 2, m, k, k, static_cast<uint32_t>(p.a_rows), S::kBK, true);
+  if (st == BEAM_OK) st = encode_tmap_2d(&p.tm_gate, Bg, 2, f, k, k, static_cast<uint32_t>(p.width), S::kBK, true);
+  if (st == BEAM_OK) st = encode_tmap_2d(&p.tm_up, Bu, 2, f, k, k, static_cast<uint32_t>(p.width), S::kBK, true);
+  if (kCta == 2) {
+    for (int i = 0; i < 3 && st == BEAM_OK; ++i)
+      if (p.out[i]) st = encode_tmap_2d_sw64(&p.tm_out[i], p.out[i], m, f, f, 32, 32);
+  }
+  if (st != BEAM_OK) return st;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  const int clusters = tiles < resident ? static_cast<int>(tiles) : resident;
+  const int smem = p.stages * p.stage_bytes + S::kStagingBytes + S::kBarBytes + 1024;
+  return launch_dependent(gated_umma_kernel<kCta>, clusters * kCta, S::kThreads, smem, kCta, stream,
+                          "cudaLaunchKernelEx(gated_umma)", p);
+}
+
+int check_sizes(int m, int n, int k) {
+  if (m <= 0 || n <= 0 || k <= 0) return BEAM_ERR_INVALID_ARG;
+  if (k % 8 != 0 || n % 8 != 0) return BEAM_ERR_ALIGNMENT;
+  // tiles are counted in 32 bits
+  if (static_cast<long long>(ceil_div(m, 128)) * ceil_div(n, 8) > (1ll << 30)) return BEAM_ERR_UNSUPPORTED;
+  return BEAM_OK;
+}
+
+}  // namespace
+
+int launch_gated(const void* A, const void* Bg, const void* Bu, void* C, void* G, void* U, int m, int f, int k,
+                 int activation, int bf16, cudaStream_t stream) {
+  if (!A || !Bg || !Bu || !C || (G == nullptr) != (U == nullptr)) return BEAM_ERR_INVALID_ARG;
+  if (activation < kActSilu || activation > kActRelu) return BEAM_ERR_INVALID_ARG;
+  int st = check_sizes(m, f, k);
+  if (st != BEAM_OK) return st;
+  if (!aligned16(A) || !aligned16(Bg) || !aligned16(Bu) || !aligned16(C) || !aligned16(G) || !aligned16(U))
+    return BEAM_ERR_ALIGNMENT;
+  const size_t ab = 2ull * m * k, bb = 2ull * f * k, cb = 2ull * m * f;
+  const void* outs[3] = {C, G, U};
+  for (int i = 0; i < 3; ++i) {
+    if (overlap(outs[i], cb, A, ab) || overlap(outs[i], cb, Bg, bb) || overlap(outs[i], cb, Bu, bb) ||
+        overlap(outs[i], cb, outs[(i + 1) % 3], cb))
+      return BEAM_ERR_INVALID_ARG;
+  }
+  DeviceCtx* ctx = current_device_ctx(&st);
+  if (!ctx) return st;
+  static ResidentTable table[2];
+  int fit[2];
+  st = resident_grid(&table[0], gated_umma_kernel<1>, ctx, GatedShape<1>::kThreads, GatedShape<1>::kSmemLimit, 1, &fit[0]);
+  if (st == BEAM_OK)
+    st = resident_grid(&table[1], gated_umma_kernel<2>, ctx, GatedShape<2>::kThreads, GatedShape<2>::kSmemLimit, 2,
+                       &fit[1]);
+  if (st != BEAM_OK) return st;
+  const GatedPlan plan = gated_plan(m, f, fit[0], fit[1]);
+  return plan.ctas == 1
+             ? launch_gated_instance<1>(ctx, plan, fit[0], A, Bg, Bu, C, G, U, m, f, k, activation, bf16, stream)
+             : launch_gated_instance<2>(ctx, plan, fit[1], A, Bg, Bu, C, G, U, m, f, k, activation, bf16, stream);
+}
+
+namespace {
+
+// Fills in one job of a gradient launch and appends its tiles to the list.
+struct JobSpec {
+  const void* a[2];
+  const void* b[2];
+  void* c;
+  int rows, cols, contraction, segments;
+  bool a_mn;
+};
+
+int add_job(GradParams* p, const JobSpec& s) {
+  GradJob& job = p->job[p->jobs];
+  for (int i = 0; i < s.segments; ++i) {
+    int st = s.a_mn ? encode_tmap_2d(&job.tm_a[i], s.a[i], 2, s.contraction, s.rows, s.rows, 64, 64, true)
+                    : encode_tmap_2d(&job.tm_a[i], s.a[i], 2, s.rows, s.contraction, s.contraction, 128, 64, true);
+    if (st == BEAM_OK) st = encode_tmap_2d(&job.tm_b[i], s.b[i], 2, s.contraction, s.cols, s.cols, 64, 64, true);
+    if (st != BEAM_OK) return st;
+  }
+  const int st = encode_tmap_2d(&job.tm_c, s.c, 2, s.rows, s.cols, s.cols, 32, 64, true);
+  if (st != BEAM_OK) return st;
+  job.rows = s.rows;
+  job.cols = s.cols;
+  job.contraction = s.contraction;
+  job.segments = s.segments;
+  job.a_mn = s.a_mn ? 1 : 0;
+  job.m_tiles = ceil_div(s.rows, 256);
+  job.n_tiles = ceil_div(s.cols, 256);
+  job.first_tile = p->tiles;
+  p->tiles += job.m_tiles * job.n_tiles;
+  ++p->jobs;
+  return BEAM_OK;
+}
+
+int launch_grad(DeviceCtx* ctx, GradParams* p, cudaStream_t stream) {
+  static ResidentTable table;
+  int fit = 0;
+  const int st = resident_grid(&table, grad_umma_kernel, ctx, GradShape::kThreads, GradShape::kSmemBytes, 2, &fit);
+  if (st != BEAM_OK) return st;
+  p->group_m = 8;
+  p->status = ctx->status_word;
+  const int clusters = p->tiles < fit ? p->tiles : fit;
+  return launch_dependent(grad_umma_kernel, clusters * 2, GradShape::kThreads, GradShape::kSmemBytes, 2, stream,
+                          "cudaLaunchKernelEx(grad_umma)", *p);
+}
+
+size_t slope_bytes(int m, int f) { return (2ull * m * f + 255) / 256 * 256; }
+
+template <bool kBf16>
+int launch_slope(DeviceCtx* ctx, const GatedSlopeParams& p, cudaStream_t stream) {
+  long long blocks = (p.count8 + 255) / 256;
+  const long long most = 8ll * ctx->sm_count;  // 2048 threads on every SM
+  if (blocks > most) blocks = most;
+  auto run = [&](auto kernel) {
+    return launch_dependent(kernel, static_cast<int>(blocks), 256, 0, 1, stream, "cudaLaunchKernelEx(gated_slope)", p);
+  };
+  switch (p.act) {
+    case kActSilu: return run(gated_slope_kernel<kActSilu, kBf16>);
+    case kActGelu: return run(gated_slope_kernel<kActGelu, kBf16>);
+    case kActGeluTanh: return run(gated_slope_kernel<kActGeluTanh, kBf16>);
+    default: return run(gated_slope_kernel<kActRelu, kBf16>);
+  }
+}
+
+}  // namespace
+
+size_t gated_backward_workspace_bytes(int m, int f) { return m > 0 && f > 0 ? 2 * slope_bytes(m, f) : 0; }
+
+int launch_gated_backward(const void* dC, const void* A, const void* Bg, const void* Bu, const void* G, const void* U,
+                          void* dA, void* dBg, void* dBu, int m, int f, int k, int activation, int bf16,
+                          void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (!dC || !G || !U || (!dA && !dBg && !dBu)) return BEAM_ERR_INVALID_ARG;
+  if (dA && (!Bg || !Bu)) return BEAM_ERR_INVALID_ARG;
+  if ((dBg || dBu) && !A) return BEAM_ERR_INVALID_ARG;
+  if (activation < kActSilu || activation > kActRelu) return BEAM_ERR_INVALID_ARG;
+  int st = check_sizes(m, f, k);
+  if (st == BEAM_OK) st = check_sizes(f, k, f);
+  if (st != BEAM_OK) return st;
+  const void* all[] = {dC, A, Bg, Bu, G, U, dA, dBg, dBu, workspace};
+  for (const void* q : all)
+    if (!aligned16(q)) return BEAM_ERR_ALIGNMENT;
+  if (!workspace || workspace_bytes < gated_backward_workspace_bytes(m, f)) return BEAM_ERR_WORKSPACE;
+  const size_t mk = 2ull * m * k, fk = 2ull * f * k, mf = 2ull * m * f;
+  const size_t bytes[] = {mf, mk, fk, fk, mf, mf, mk, fk, fk, gated_backward_workspace_bytes(m, f)};
+  for (int o = 6; o < 10; ++o)
+    for (int i = 0; i < o; ++i)
+      if (overlap(all[o], bytes[o], all[i], bytes[i])) return BEAM_ERR_INVALID_ARG;
+  DeviceCtx* ctx = current_device_ctx(&st);
+  if (!ctx) return st;
+
+  uint8_t* dG = static_cast<uint8_t*>(workspace);
+  uint8_t* dU = dG + slope_bytes(m, f);
+  GatedSlopeParams sp = {};
+  sp.dc = static_cast<const uint4*>(dC);
+  sp.gate = static_cast<const uint4*>(G);
+  sp.up = static_cast<const uint4*>(U);
+  sp.dgate = reinterpret_cast<uint4*>(dG);
+  sp.dup = reinterpret_cast<uint4*>(dU);
+  sp.count8 = static_cast<long long>(m) * (f / 8);
+  sp.act = activation;
+
+  GradParams p = {};
+  p.bf16 = bf16;
+  if (dA) st = add_job(&p, {{dG, dU}, {Bg, Bu}, dA, m, k, f, 2, false});
+  if (st == BEAM_OK && dBg) st = add_job(&p, {{dG, nullptr}, {A, nullptr}, dBg, f, k, m, 1, true});
+  if (st == BEAM_OK && dBu) st = add_job(&p, {{dU, nullptr}, {A, nullptr}, dBu, f, k, m, 1, true});
+  if (st != BEAM_OK) return st;
+  st = bf16 ? launch_slope<true>(ctx, sp, stream) : launch_slope<false>(ctx, sp, stream);
+  if (st != BEAM_OK) return st;
+  return launch_grad(ctx, &p, stream);
+}
+
+int launch_gemmrc_backward(const void* dC, const void* A, const void* B, void* dA, void* dB, int m, int n, int k,
+                           int bf16, cudaStream_t stream) {
+  if (!dC || (!dA && !dB) || (dA && !B) || (dB && !A)) return BEAM_ERR_INVALID_ARG;
+  int st = check_sizes(m, n, k);
+  if (st == BEAM_OK) st = check_sizes(n, k, n);
+  if (st != BEAM_OK) return st;
+  const void* all[] = {dC, A, B, dA, dB};
+  for (const void* q : all)
+    if (!aligned16(q)) return BEAM_ERR_ALIGNMENT;
+  const size_t mk = 2ull * m * k, nk = 2ull * n * k, mn = 2ull * m * n;
+  const size_t bytes[] = {mn, mk, nk, mk, nk};
+  for (int o = 3; o < 5; ++o)
+    for (int i = 0; i < o; ++i)
+      if (overlap(all[o], bytes[o], all[i], bytes[i])) return BEAM_ERR_INVALID_ARG;
+  DeviceCtx* ctx = current_device_ctx(&st);
+  if (!ctx) return st;
+  GradParams p = {};
+  p.bf16 = bf16;
+  const JobSpec da = {{dC, nullptr}, {B, nullptr}, dA, m, k, n, 1, false};
+  const JobSpec db = {{dC, nullptr}, {A, nullptr}, dB, n, k, m, 1, true};
+  const bool da_first = n >= m;  // the longer contraction first
+  if (dA && da_first) st = add_job(&p, da);
+  if (st == BEAM_OK && dB) st = add_job(&p, db);
+  if (st == BEAM_OK && dA && !da_first) st = add_job(&p, da);
+  if (st != BEAM_OK) return st;
+  return launch_grad(ctx, &p, stream);
+}
+
+}  // namespace beam

@@ -1,0 +1,351 @@
+// The gated product of a feed-forward block as one kernel:
+//
+//   G = A Bg^T,  U = A Bu^T,  C = act(G) * U        A [M, K], Bg and Bu [F, K], C [M, F], fp16 or bf16
+//
+// A tile is 128 kCta rows by `width` columns of BOTH products.  The two weights enter one UMMA as the halves of its
+// N = 2 * width rows of B: on a CTA pair (kCta = 2) the leader CTA loads `width` rows of Bg and its peer the same rows
+// of Bu, which is how a cta_group::2 UMMA splits B anyway; a single CTA loads both boxes one behind the other.  So the
+// main loop is that of the plain rc GEMM (gemmrc_umma.cuh) with nothing added, A is read once for both products, and
+// column j of G and of U stand in TMEM columns j and width + j of the same lane: the epilogue multiplies them in
+// registers and G and U never leave the SM, unless the caller wants them kept for the backward pass.  The products are
+// accumulated and combined in fp32 and rounded once to the output type (three times, independently, when kept).
+//
+// Two variants, chosen by rows (the rule and what it measured stand beside gated_plan() in feedforward_launch.cu):
+//   kCta = 2   M > 128: 256-row tiles, width 32, 64, 96 or 128, persistent grid, two TMEM accumulators, C stored by TMA.
+//   kCta = 1   M <= 128: the call is bound by reading the weights once.  The width is whatever multiple of 8 deals F
+//              to all SMs in one wave, so that every SM streams the same share of the weights through a ring of up to 8
+//              stages; only the rows of A that exist are loaded (the other lanes of the UMMA compute on leftovers that
+//              are never stored); C is small and written straight from registers.
+//
+// Roles: warp 0 TMA producer, warp 1 MMA issuer, warps 2..5 epilogue.
+#pragma once
+
+#include "activation.cuh"
+#include "umma_common.cuh"
+
+namespace beam {
+
+struct GatedParams {
+  CUtensorMap tm_a;       // A [M, K], box (rows per CTA) x 64, 128 B swizzle
+  CUtensorMap tm_gate;    // Bg [F, K], box width x 64
+  CUtensorMap tm_up;      // Bu [F, K]
+  CUtensorMap tm_out[3];  // pair variant: C, G, U [M, F], store box 32 rows x 32 columns, 64 B swizzle
+  void* out[3];           // C, G, U; G and U are null when they are not kept
+  int m, f, k;
+  int width;              // columns of F per tile
+  int a_rows;             // rows of A that a CTA loads
+  int stages, stage_bytes;
+  int m_tiles, n_tiles, group_m;
+  int act;
+  int bf16;
+  int* status;
+};
+
+template <int kCta>
+struct GatedShape {
+  static constexpr int kBM = 128;
+  static constexpr int kBK = 64;
+  static constexpr int kABytes = kBM * kBK * 2;
+  static constexpr int kMaxStages = 8;
+  static constexpr int kThreads = 192;
+  static constexpr int kAccCols = 256;  // TMEM columns between the two accumulators
+  static constexpr int kBufsPerWarp = 4;
+  static constexpr int kStoreBufBytes = 32 * 64;
+  static constexpr int kStagingBytes = kCta == 2 ? 4 * kBufsPerWarp * kStoreBufBytes : 0;
+  static constexpr int kBarBytes = 256;
+  static constexpr int kSmemLimit = 232448;
+  static constexpr int kRingBytes = kSmemLimit - 1024 - kStagingBytes - kBarBytes;
+  static_assert((2 * kMaxStages + 4) * 8 + 8 <= kBarBytes, "barrier block too small");
+};
+
+template <int kAct>
+__device__ __forceinline__ void gated_combine(uint32_t (&g)[32], const uint32_t (&u)[32]) {
+#pragma unroll
+  for (int q = 0; q < 32; ++q)
+    g[q] = __float_as_uint(act_value<kAct>(__uint_as_float(g[q])) * __uint_as_float(u[q]));
+}
+__device__ __forceinline__ void gated_combine(int act, uint32_t (&g)[32], const uint32_t (&u)[32]) {
+  switch (act) {  // warp-uniform
+    case kActSilu: gated_combine<kActSilu>(g, u); break;
+    case kActGelu: gated_combine<kActGelu>(g, u); break;
+    case kActGeluTanh: gated_combine<kActGeluTanh>(g, u); break;
+    default: gated_combine<kActRelu>(g, u); break;
+  }
+}
+
+template <int kCta>
+__global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
+    gated_umma_kernel(const __grid_constant__ GatedParams p) {
+  using S = GatedShape<kCta>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t cta_rank = (kCta == 2) ? ptx::cluster_ctarank() : 0u;
+  const bool leader = cta_rank == 0;
+  const int first = static_cast<int>(blockIdx.x) / kCta;
+  const int stride = static_cast<int>(gridDim.x) / kCta;
+  const int tiles = p.m_tiles * p.n_tiles;
+  const int num_kb = (p.k + S::kBK - 1) / S::kBK;
+
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const uint32_t ring_bytes = static_cast<uint32_t>(p.stages * p.stage_bytes);
+  const uint32_t staging_base = smem_base + ring_bytes;
+  const uint32_t bar_base = staging_base + S::kStagingBytes;
+  auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (S::kMaxStages + s); };
+  auto tmem_full_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + a); };
+  auto tmem_empty_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + 2 + a); };
+  volatile uint32_t* tmem_slot =
+      reinterpret_cast<volatile uint32_t*>(smem_gen + ring_bytes + S::kStagingBytes + 8 * (2 * S::kMaxStages + 4));
+  volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  // Groups of group_m row tiles are walked column-major, so tiles in flight together share rows of A and of the weights.
+  auto tile_at = [&](int t, int& mt, int& nt) {
+    const int per_group = p.group_m * p.n_tiles;
+    const int g = t / per_group;
+    const int first_m = g * p.group_m;
+    const int rows = min(p.group_m, p.m_tiles - first_m);
+    const int r = t - g * per_group;
+    mt = first_m + r % rows;
+    nt = r / rows;
+  };
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < static_cast<uint32_t>(p.stages); ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (uint32_t a = 0; a < 2; ++a) {
+      ptx::mbar_init(tmem_full_bar(a), 1);
+      ptx::mbar_init(tmem_empty_bar(a), 4 * kCta);  // one arrive per epilogue warp of each CTA
+    }
+    *cta_abort = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&p.tm_a);
+    ptx::prefetch_tensormap(&p.tm_gate);
+    ptx::prefetch_tensormap(&p.tm_up);
+    ptx::grid_launch_dependents();  // the next kernel on the stream may set itself up; it waits for this grid itself
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<kCta>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    ptx::tmem_relinquish<kCta>();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (kCta == 2) ptx::cluster_sync_all();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      ptx::grid_dependency_wait();  // before the first global read; everything else follows from these reads
+      const uint32_t b_bytes = static_cast<uint32_t>(p.width) * 128u;
+      const uint32_t bytes = 2u * b_bytes + static_cast<uint32_t>(kCta) * static_cast<uint32_t>(p.a_rows) * 128u;
+      uint32_t s = 0, ph = 0;
+      bool alive = true;
+      for (int t = first; alive && t < tiles; t += stride) {
+        int mt, nt;
+        tile_at(t, mt, nt);
+        const int row_a = (mt * kCta + static_cast<int>(cta_rank)) * S::kBM;
+        const int row_b = nt * p.width;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!bounded_wait(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait)) {
+            alive = false;
+            break;
+          }
+          const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
+          const uint32_t b = a + S::kABytes;
+          if (leader) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
+          if constexpr (kCta == 2) {
+            const uint32_t bar = ptx::mapa(full_bar(s), 0);
+            ptx::tma_load_2d_pair(a, &p.tm_a, bar, kb * S::kBK, row_a);
+            ptx::tma_load_2d_pair(b, leader ? &p.tm_gate : &p.tm_up, bar, kb * S::kBK, row_b);
+          } else {
+            ptx::tma_load_2d(b, &p.tm_gate, full_bar(s), kb * S::kBK, row_b);
+            ptx::tma_load_2d(b + b_bytes, &p.tm_up, full_bar(s), kb * S::kBK, row_b);
+            ptx::tma_load_2d(a, &p.tm_a, full_bar(s), kb * S::kBK, row_a);
+          }
+          if (++s == static_cast<uint32_t>(p.stages)) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0 && leader) {
+      const uint32_t idesc =
+          ptx::umma_idesc_f16_f32(S::kBM * kCta, 2 * p.width) | (p.bf16 ? ptx::kIdescBf16Inputs : 0u);
+      const uint64_t a_desc0 = ptx::umma_desc_k_sw128(smem_base);
+      const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + S::kABytes);
+      const uint64_t desc_stride = static_cast<uint64_t>(p.stage_bytes >> 4);
+      uint32_t s = 0, ph = 0;
+      bool alive = true;
+      for (int t = first, j = 0; alive && t < tiles; t += stride, ++j) {
+        const uint32_t acc = static_cast<uint32_t>(j) & 1u;
+        const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
+        if (!bounded_wait(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc)) break;
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * S::kAccCols;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!bounded_wait(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull)) {
+            alive = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          ptx::umma_f16_kblock<kCta>(d_tmem, a_desc0 + s * desc_stride, b_desc0 + s * desc_stride, idesc,
+                                     kb > 0 ? 1u : 0u);
+          if constexpr (kCta == 1)
+            ptx::umma_commit<1>(empty_bar(s));
+          else
+            ptx::umma_commit_pair_both(empty_bar(s), 0x3);
+          if (++s == static_cast<uint32_t>(p.stages)) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (alive) {
+          if constexpr (kCta == 1)
+            ptx::umma_commit<1>(tmem_full_bar(acc));
+          else
+            ptx::umma_commit_pair_both(tmem_full_bar(acc), 0x3);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue (warps 2..5)
+    const uint32_t quad = warp & 3u;  // TMEM lanes [32 quad, 32 quad + 32) are this warp's to read
+    const uint32_t lead_empty0 = (kCta == 2) ? ptx::mapa(tmem_empty_bar(0), 0) : tmem_empty_bar(0);
+    const bool keep = p.out[1] != nullptr;
+    uint32_t stores = 0;  // bulk stores this warp has issued (selects the staging buffer)
+    for (int t = first, j = 0; t < tiles; t += stride, ++j) {
+      const uint32_t acc = static_cast<uint32_t>(j) & 1u;
+      const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
+      if (!bounded_wait_warp(tmem_full_bar(acc), acc_ph, cta_abort, p.status, kFaultEpilogueWait, lane)) break;
+      ptx::tc_fence_after();
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int row0 = (mt * kCta + static_cast<int>(cta_rank)) * S::kBM + static_cast<int>(quad) * 32;
+      const int col0 = nt * p.width;
+      const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * S::kAccCols;
+      const bool rows_live = row0 < p.m;  // warp-uniform
+      for (int c = 0; rows_live && c < p.width && col0 + c < p.f; c += 32) {
+        uint32_t g[32], u[32];
+        ptx::tmem_ld_32x32(taddr + c, g);  // a narrow tile's last read runs into the neighbouring columns: not stored
+        ptx::tmem_ld_32x32(taddr + p.width + c, u);
+        ptx::tmem_ld_wait();
+        // Writes 32 columns of output `which`, rounded once.
+        auto store = [&](const uint32_t(&v)[32], int which) {
+          uint32_t o[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            o[q] = ptx::pack_out2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]), p.bf16);
+          if constexpr (kCta == 2) {
+            // `width` is a multiple of 32 here, so a box never reaches into the next tile's columns.
+            const uint32_t buf =
+                staging_base + (quad * S::kBufsPerWarp + stores % S::kBufsPerWarp) * S::kStoreBufBytes;
+            if (stores >= S::kBufsPerWarp) {
+              if (lane == 0) ptx::tma_store_wait_read<S::kBufsPerWarp - 1>();
+              __syncwarp();
+            }
+            // Row `lane` of the box, 16-byte piece i at i ^ (lane / 2 % 4): the 64-byte swizzle, free of bank conflicts.
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              ptx::st_shared_v4(buf + lane * 64u + ((static_cast<uint32_t>(i) ^ ((lane >> 1) & 3u)) << 4), o[4 * i],
+                                o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              ptx::tma_store_2d(&p.tm_out[which], buf, col0 + c, row0);
+              ptx::tma_store_commit();
+            }
+            ++stores;
+          } else {
+            const int row = row0 + static_cast<int>(lane);
+            const int valid = min(min(32, p.width - c), p.f - (col0 + c));  // a multiple of 8
+            if (row < p.m) {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out[which]) +
+                                                    (static_cast<size_t>(row) * p.f + col0 + c) * 2);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (8 * i < valid) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          }
+        };
+        if (keep) {
+          store(g, 1);
+          store(u, 2);
+        }
+        gated_combine(p.act, g, u);
+        store(g, 0);
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kCta == 1)
+          ptx::mbar_arrive(tmem_empty_bar(acc));
+        else
+          ptx::mbar_arrive_cluster(lead_empty0 + 8u * acc);
+      }
+    }
+  }
+
+  // ---- teardown: bulk stores have read their staging buffers; then everyone meets and the allocating warp frees TMEM
+  if (kCta == 2 && warp >= 2 && lane == 0) ptx::tma_store_wait_read<0>();
+  __syncwarp();
+  if (*cta_abort) abort_drain_delay();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (kCta == 2) ptx::cluster_sync_all();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<kCta>(tmem_base, 512);
+  }
+}
+
+// dG = dC * U * act'(G) and dU = dC * act(G), element by element in fp32, rounded once to the operands' type: they are
+// operands of the four products of the backward pass, which the tensor cores take in 16 bits.  Bound by memory: 10 bytes
+// per element; 8 elements per thread keep three 16-byte loads in flight.
+struct GatedSlopeParams {
+  const uint4* dc;
+  const uint4* gate;
+  const uint4* up;
+  uint4* dgate;
+  uint4* dup;
+  long long count8;  // groups of 8 elements
+  int act;
+  int bf16;
+};
+
+template <int kAct, bool kBf16>
+__device__ __forceinline__ void gated_slope8(const uint4& d4, const uint4& g4, const uint4& u4, uint4& dg4, uint4& du4) {
+  const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w}, g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+  uint32_t dg[4], du[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 df = ptx::unpack_in2(d[i], kBf16), gf = ptx::unpack_in2(g[i], kBf16), uf = ptx::unpack_in2(u[i], kBf16);
+    const float2 lo = act_value_slope<kAct>(gf.x), hi = act_value_slope<kAct>(gf.y);
+    dg[i] = ptx::pack_out2(df.x * uf.x * lo.y, df.y * uf.y * hi.y, kBf16);
+    du[i] = ptx::pack_out2(df.x * lo.x, df.y * hi.x, kBf16);
+  }
+  dg4 = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+  du4 = make_uint4(du[0], du[1], du[2], du[3]);
+}
+
+template <int kAct, bool kBf16>
+__global__ void __launch_bounds__(256) gated_slope_kernel(const GatedSlopeParams p) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  const long long stride = static_cast<long long>(gridDim.x) * 256;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < p.count8; i += stride) {
+    uint4 dg, du;
+    gated_slope8<kAct, kBf16>(__ldcs(p.dc + i), __ldcs(p.gate + i), __ldcs(p.up + i), dg, du);
+    p.dgate[i] = dg;  // read again by the products that follow: the default policy leaves them in L2 where they fit
+    p.dup[i] = du;
+  }
+}
+
+}  // namespace beam

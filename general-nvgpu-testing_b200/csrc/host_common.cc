@@ -119,10 +119,12 @@ DeviceCtx* current_device_ctx(int* err) {
   return c;
 }
 
-int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t ld,
-                   uint32_t box_rows, uint32_t box_cols, bool swizzle128) {
+namespace {
+
+int encode_2d(CUtensorMap* out, const void* base, CUtensorMapDataType type, int elem_bytes, uint64_t rows,
+              uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swizzle) {
   const TmapKey key = {base, cols, rows, 0, ld, box_cols, box_rows,
-                       static_cast<uint32_t>(elem_bytes) | (swizzle128 ? 0x100u : 0u)};
+                       static_cast<uint32_t>(elem_bytes) | (static_cast<uint32_t>(swizzle) << 8)};
   if (tmap_lookup(key, out)) return BEAM_OK;
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return BEAM_ERR_TENSORMAP;
@@ -130,10 +132,8 @@ int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t 
   const cuuint64_t gstride[1] = {ld * static_cast<uint64_t>(elem_bytes)};
   const cuuint32_t box[2] = {box_cols, box_rows};
   const cuuint32_t estride[2] = {1, 1};
-  const CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  CUresult r = fn(out, dt, 2, const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = fn(out, type, 2, const_cast<void*>(base), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     std::snprintf(t_cuda_error, sizeof(t_cuda_error), "cuTensorMapEncodeTiled failed with CUresult %d",
                   static_cast<int>(r));
@@ -141,6 +141,33 @@ int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t 
   }
   tmap_remember(key, out);
   return BEAM_OK;
+}
+
+}  // namespace
+
+int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t ld,
+                   uint32_t box_rows, uint32_t box_cols, bool swizzle128) {
+  return encode_2d(out, base, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                   elem_bytes, rows, cols, ld, box_rows, box_cols,
+                   swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+int encode_tmap_2d_sw64(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                        uint32_t box_rows, uint32_t box_cols) {
+  return encode_2d(out, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, rows, cols, ld, box_rows, box_cols,
+                   CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+int encode_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                      uint32_t box_cols) {
+  return encode_2d(out, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, cols, cols, box_rows, box_cols,
+                   CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int encode_tmap_2d_words64(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                           uint32_t box_cols) {
+  return encode_2d(out, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 8, rows, cols, cols, box_rows, box_cols,
+                   CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // 3-D row-major fp32 tensor [planes][rows][cols] (dense), box = 1 x box_rows x box_cols, 128-byte swizzle.

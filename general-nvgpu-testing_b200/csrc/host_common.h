@@ -34,6 +34,15 @@ DeviceCtx* current_device_ctx(int* err);
 int encode_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, uint64_t rows, uint64_t cols, uint64_t ld,
                    uint32_t box_rows, uint32_t box_cols, bool swizzle128);
 
+// 16-bit elements, 64-byte swizzle (box_cols * 2 = 64 B); packed bytes, 128-byte swizzle (box_cols = 128); and 8-byte
+// words without a swizzle, for tables whose rows are copied as they are.
+int encode_tmap_2d_sw64(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                        uint32_t box_rows, uint32_t box_cols);
+int encode_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                      uint32_t box_cols);
+int encode_tmap_2d_words64(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
+                           uint32_t box_cols);
+
 // Dense 3-D fp32 tensor [planes][rows][cols], box 1 x box_rows x box_cols (box_cols * 4 = 128 B), 128-byte swizzle.
 int encode_tmap_3d_f32(CUtensorMap* out, const void* base, uint64_t planes, uint64_t rows, uint64_t cols,
                        uint32_t box_rows, uint32_t box_cols);

@@ -1,0 +1,145 @@
+// Host launchers of MXFP4 quantisation and product.
+#include "mxfp4_launch.h"
+
+#include "launch_common.h"
+#include "mxfp4_umma.cuh"
+
+namespace beam {
+
+namespace {
+
+int check_matrix(int rows, int k) {
+  if (rows <= 0 || k <= 0) return BEAM_ERR_INVALID_ARG;
+  if (k % 32 != 0) return BEAM_ERR_ALIGNMENT;
+  // units of 128 elements are counted in 32 bits
+  if (static_cast<long long>(ceil_div(rows, 128)) * 128 * ceil_div(k, 128) > (1ll << 31) - 1024)
+    return BEAM_ERR_UNSUPPORTED;
+  return BEAM_OK;
+}
+
+size_t packed_bytes(int rows, int k) { return static_cast<size_t>(rows) * (k / 2); }
+
+struct Units {
+  uint32_t kblocks, units;
+  int grid;
+};
+Units count_units(int rows, int k) {
+  Units u;
+  u.kblocks = static_cast<uint32_t>(ceil_div(k, 128));
+  u.units = static_cast<uint32_t>(rows) * u.kblocks;
+  u.grid = static_cast<int>((u.units + 16 * kMxUnits - 1) / (16 * kMxUnits));
+  return u;
+}
+
+// Columns per tile for M <= 128: B is read once whatever the width, so the width only deals out N.  64 or 128: a tile's scales
+// start at the first or the third of the four TMEM columns of a scale block, and a UMMA takes scales from even columns only
+// (a width of 32, which starts every other tile at an odd column, faulted with a misaligned address).
+int narrow_width(int n, int sm_count) { return ceil_div(n, 64) <= sm_count ? 64 : 128; }
+
+template <int kCta>
+int launch_instance(DeviceCtx* ctx, const void* A, const void* sa, const void* B, const void* sb, void* C, int m, int n,
+                    int k, int bf16, cudaStream_t stream) {
+  using S = MxShape<kCta>;
+  static ResidentTable table;
+  int resident = 0;
+  int st = resident_grid(&table, mxfp4_umma_kernel<kCta>, ctx, S::kThreads, S::kSmemLimit, kCta, &resident);
+  if (st != BEAM_OK) return st;
+  MxGemmParams p = {};
+  p.c = C;
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.bf16 = bf16;
+  p.status = ctx->status_word;
+  p.width = kCta == 2 ? S::kMaxWidth : narrow_width(n, resident);
+  p.a_rows = kCta == 2 ? 128 : (m + 7) / 8 * 8;
+  p.stage_bytes = S::kABytes + p.width / kCta * 128 + S::kScaleBytes;
+  p.stages = S::kRingBytes / p.stage_bytes;
+  if (p.stages > S::kMaxStages) p.stages = S::kMaxStages;
+  p.m_tiles = ceil_div(m, 128 * kCta);
+  p.n_tiles = ceil_div(n, p.width);
+  p.group_m = 8;
+  const uint64_t words = 64ull * ceil_div(k, 128);
+  st = encode_tmap_2d_u8(&p.tm_a, A, m, k / 2, static_cast<uint32_t>(p.a_rows), 128);
+  if (st == BEAM_OK) st = encode_tmap_2d_u8(&p.tm_b, B, n, k / 2, static_cast<uint32_t>(p.width / kCta), 128);
+  if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sa, sa, ceil_div(m, 128), words, 1, 128);
+  if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sb, sb, ceil_div(n, 128), words, 2, 128);
+  if (st == BEAM_OK && kCta == 2) st = encode_tmap_2d(&p.tm_c, C, 2, m, n, n, 32, 64, true);
+  if (st != BEAM_OK) return st;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  const int clusters = tiles < resident ? static_cast<int>(tiles) : resident;
+  const int smem = p.stages * p.stage_bytes + S::kStagingBytes + S::kBarBytes + 1024;
+  return launch_dependent(mxfp4_umma_kernel<kCta>, clusters * kCta, S::kThreads, smem, kCta, stream,
+                          "cudaLaunchKernelEx(mxfp4_umma)", p);
+}
+
+}  // namespace
+
+size_t mxfp4_scales_bytes(int rows, int k) {
+  if (rows <= 0 || k <= 0) return 0;
+  return 512ull * ceil_div(rows, 128) * ceil_div(k, 128);
+}
+
+int launch_mxfp4_quantize(const void* x, void* q, void* scales, int rows, int k, int bf16, cudaStream_t stream) {
+  if (!x || !q || !scales) return BEAM_ERR_INVALID_ARG;
+  int st = check_matrix(rows, k);
+  if (st != BEAM_OK) return st;
+  if (!aligned16(x) || !aligned16(q) || !aligned16(scales)) return BEAM_ERR_ALIGNMENT;
+  const size_t xb = 2ull * rows * k, qb = packed_bytes(rows, k), sb = mxfp4_scales_bytes(rows, k);
+  if (overlap(x, xb, q, qb) || overlap(x, xb, scales, sb) || overlap(q, qb, scales, sb)) return BEAM_ERR_INVALID_ARG;
+  DeviceCtx* ctx = current_device_ctx(&st);
+  if (!ctx) return st;
+  const Units u = count_units(ceil_div(rows, 128) * 128, k);
+  MxQuantParams p = {};
+  p.x = static_cast<const uint4*>(x);
+  p.q = static_cast<uint32_t*>(q);
+  p.scales = static_cast<uint32_t*>(scales);
+  p.rows = rows;
+  p.k = k;
+  p.kblocks = u.kblocks;
+  p.units = u.units;
+  p.bf16 = bf16;
+  return launch_dependent(bf16 ? mxfp4_quantize_kernel<true> : mxfp4_quantize_kernel<false>, u.grid, 256, 0, 1, stream,
+                          "cudaLaunchKernelEx(mxfp4_quantize)", p);
+}
+
+int launch_mxfp4_dequantize(const void* q, const void* scales, void* x, int rows, int k, int type, cudaStream_t stream) {
+  if (!x || !q || !scales) return BEAM_ERR_INVALID_ARG;
+  int st = check_matrix(rows, k);
+  if (st != BEAM_OK) return st;
+  if (!aligned16(x) || !aligned16(q) || !aligned16(scales)) return BEAM_ERR_ALIGNMENT;
+  const size_t xb = (type == kMxFp32 ? 4ull : 2ull) * rows * k;
+  if (overlap(x, xb, q, packed_bytes(rows, k)) || overlap(x, xb, scales, mxfp4_scales_bytes(rows, k)))
+    return BEAM_ERR_INVALID_ARG;
+  DeviceCtx* ctx = current_device_ctx(&st);
+  if (!ctx) return st;
+  const Units u = count_units(rows, k);
+  auto kernel = type == kMxFp32   ? mxfp4_dequantize_kernel<kMxFp32>
+                : type == kMxBf16 ? mxfp4_dequantize_kernel<kMxBf16>
+                                  : mxfp4_dequantize_kernel<kMxFp16>;
+  return launch_dependent(kernel, u.grid, 256, 0, 1, stream, "cudaLaunchKernelEx(mxfp4_dequantize)",
+                          static_cast<const uint32_t*>(q), static_cast<const uint32_t*>(scales), static_cast<uint4*>(x),
+                          rows, k, u.kblocks, u.units);
+}
+
+int launch_mxfp4_gemmrc(const void* A, const void* a_scales, const void* B, const void* b_scales, void* C, int m, int n,
+                        int k, int bf16, cudaStream_t stream) {
+  if (!A || !a_scales || !B || !b_scales || !C) return BEAM_ERR_INVALID_ARG;
+  int st = check_matrix(m, k);
+  if (st == BEAM_OK) st = check_matrix(n, k);
+  if (st != BEAM_OK) return st;
+  if (n % 8 != 0) return BEAM_ERR_ALIGNMENT;
+  if (!aligned16(A) || !aligned16(a_scales) || !aligned16(B) || !aligned16(b_scales) || !aligned16(C))
+    return BEAM_ERR_ALIGNMENT;
+  if (static_cast<long long>(ceil_div(m, 128)) * ceil_div(n, 32) > (1ll << 30)) return BEAM_ERR_UNSUPPORTED;
+  const size_t cb = 2ull * m * n;
+  if (overlap(C, cb, A, packed_bytes(m, k)) || overlap(C, cb, B, packed_bytes(n, k)) ||
+      overlap(C, cb, a_scales, mxfp4_scales_bytes(m, k)) || overlap(C, cb, b_scales, mxfp4_scales_bytes(n, k)))
+    return BEAM_ERR_INVALID_ARG;
+  DeviceCtx* ctx = current_device_ctx(&st);
+  if (!ctx) return st;
+  return m <= 128 ? launch_instance<1>(ctx, A, a_scales, B, b_scales, C, m, n, k, bf16, stream)
+                  : launch_instance<2>(ctx, A, a_scales, B, b_scales, C, m, n, k, bf16, stream);
+}
+
+}  // namespace beam

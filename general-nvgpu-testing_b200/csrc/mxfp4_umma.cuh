@@ -1,0 +1,460 @@
+// MXFP4: quantisation, its inverse, and the product C = A B^T of two quantised matrices on the 4-bit tensor cores.
+//
+// A quantised [R, K] matrix (K a multiple of 32) is two arrays:
+//   q       [R, K / 2] bytes, e2m1 codes, element 2 i in the low half of byte i;
+//   scales  one ue8m0 byte (2^(s - 127), 255 = NaN) per 32 elements of a row, in blocks of 128 rows x 4 scales,
+//           [ceil(R / 128)][ceil(K / 128)][512]: row r, scale c of a block at byte (r % 32) * 16 + (r / 32) * 4 + c.
+// The scale blocks are what the tensor cores take: 512 contiguous bytes are one copy into TMEM, so the product moves
+// scales like any other operand tile and no thread ever touches one.  Scales outside the matrix are 0.
+#pragma once
+
+#include "umma_common.cuh"
+
+namespace beam {
+
+// ------------------------------------------------------------------ quantisation
+// One half-warp takes 128 elements of a row (a row of one scale block): each lane 8 elements, four lanes a scale.
+//   s = floor(log2(max |x|)) - 2, at least -127: the exponent field of the largest magnitude, without a logarithm;
+//   q = x 2^-s rounded to the nearest e2m1 value, ties to even; magnitudes above 6 (up to 8 by the choice of s) become 6.
+// The scaling is exact in fp32.  A block with an infinity or a NaN gets the NaN scale.  Bound by memory: 2 bytes in and
+// 17/32 out per element; each thread keeps kUnits 16-byte loads in flight.
+struct MxQuantParams {
+  const uint4* x;
+  uint32_t* q;       // 8 codes per word
+  uint32_t* scales;  // 4 scales per word
+  int rows, k;
+  uint32_t kblocks;  // ceil(k / 128)
+  uint32_t units;    // rows padded to 128, times kblocks
+  int bf16;
+};
+
+constexpr int kMxUnits = 4;
+
+__device__ __forceinline__ size_t mx_scale_word(uint32_t row, uint32_t kb, uint32_t kblocks) {
+  return (static_cast<size_t>(row >> 7) * kblocks + kb) * 128 + (row & 31) * 4 + ((row >> 5) & 3);
+}
+
+template <bool kBf16>
+static __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxQuantParams p) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  const uint32_t lane = threadIdx.x & 15;
+  const uint32_t first = blockIdx.x * (16 * kMxUnits) + (threadIdx.x >> 4);
+  uint4 x[kMxUnits];
+  uint32_t row[kMxUnits], kb[kMxUnits];
+  bool live[kMxUnits];
+#pragma unroll
+  for (int i = 0; i < kMxUnits; ++i) {
+    const uint32_t u = first + 16 * i;
+    row[i] = u / p.kblocks;
+    kb[i] = u - row[i] * p.kblocks;
+    const uint32_t col = kb[i] * 128 + lane * 8;
+    live[i] = u < p.units && row[i] < static_cast<uint32_t>(p.rows) && col < static_cast<uint32_t>(p.k);
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (live[i]) x[i] = __ldcs(p.x + (static_cast<size_t>(row[i]) * p.k + col) / 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kMxUnits; ++i) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    float v[8];
+    uint32_t top = 0;  // magnitudes compare as integers; infinities and NaN above all finite values
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = ptx::unpack_in2(w[j], kBf16);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+      top = max(top, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
+    }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t field = top >> 23;
+    uint32_t scale = field > 2 ? field - 2 : 0;
+    // 2^-s: exponent field 254 - scale, between 2 and 254
+    float inv = __uint_as_float((254u - scale) << 23);
+    if (field == 255) {
+      scale = 255;
+      inv = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = field == 255 ? 0.f : v[j] * inv;
+    const uint32_t code = ptx::pack_e2m1x8(v);
+    if (live[i]) p.q[(static_cast<size_t>(row[i]) * p.k + kb[i] * 128 + lane * 8) / 8] = code;
+    // the half-warp's four scales as one word; lanes past K hold zeros and so give scale 0
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) word |= __shfl_sync(0xffffffffu, scale, j * 4, 16) << (8 * j);
+    if (lane == 0 && first + 16 * i < p.units) p.scales[mx_scale_word(row[i], kb[i], p.kblocks)] = word;
+  }
+}
+
+enum MxType : int { kMxFp16 = 0, kMxBf16 = 1, kMxFp32 = 2 };
+
+// The inverse: x = q 2^s, exact in fp32 and rounded to the output type.  Same units.
+template <int kType>
+static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* __restrict__ q,
+                                                                      const uint32_t* __restrict__ scales,
+                                                                      uint4* __restrict__ x, int rows, int k,
+                                                                      uint32_t kblocks, uint32_t units) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  const uint32_t lane = threadIdx.x & 15;
+  const uint32_t first = blockIdx.x * (16 * kMxUnits) + (threadIdx.x >> 4);
+  uint32_t code[kMxUnits], word[kMxUnits];
+  size_t at[kMxUnits];
+  bool live[kMxUnits];
+#pragma unroll
+  for (int i = 0; i < kMxUnits; ++i) {
+    const uint32_t u = first + 16 * i;
+    const uint32_t row = u / kblocks, kb = u - row * kblocks, col = kb * 128 + lane * 8;
+    live[i] = u < units && col < static_cast<uint32_t>(k);
+    at[i] = (static_cast<size_t>(row) * k + col) / 8;
+    code[i] = live[i] ? __ldcs(q + at[i]) : 0u;
+    word[i] = live[i] ? __ldg(scales + mx_scale_word(row, kb, kblocks)) : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < kMxUnits; ++i) {
+    if (!live[i]) continue;
+    const uint32_t s = (word[i] >> (8 * (lane >> 2))) & 255u;
+    // 2^(s - 127) in fp32: 0 is the subnormal 2^-127, 255 a NaN
+    const float scale = __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7FC00000u : s << 23);
+    float v[8];
+    ptx::unpack_e2m1x8(code[i], v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= scale;
+    if constexpr (kType == kMxFp32) {
+      float4* dst = reinterpret_cast<float4*>(x) + 2 * at[i];
+      __stcs(dst, make_float4(v[0], v[1], v[2], v[3]));
+      __stcs(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
+    } else {
+      __stcs(x + at[i], make_uint4(ptx::pack_out2(v[0], v[1], kType), ptx::pack_out2(v[2], v[3], kType),
+                                   ptx::pack_out2(v[4], v[5], kType), ptx::pack_out2(v[6], v[7], kType)));
+    }
+  }
+}
+
+// ------------------------------------------------------------------ product
+// C[M, N] = A B^T: 4-bit UMMAs (K = 64) with block scales, fp32 accumulation, one rounding to fp16 or bf16.
+//
+// A stage of the ring is 256 elements of K: 128 bytes per row, laid out by TMA with the 128-byte swizzle like any K-major
+// operand, and 3 KB of scale blocks (one row block for A, two for B) that a second copy brings as they are.  Per 128
+// elements the issuing thread copies three scale blocks into TMEM and issues two UMMAs; copies and UMMAs of one thread
+// execute in order, so nothing else separates them; two sets of scale columns alternate.
+//
+//   kCta = 2   256 x 256 tiles on a pair.  B's scales of all 256 columns are needed in both CTAs' TMEM, so both load them.
+//              Two accumulators of 256 columns and the scales do not fit into 512 columns, so the accumulators overlap
+//              by 64 columns: the epilogue of a tile drains that part first and hands it back, after which the next
+//              tile's UMMAs may start in the other accumulator while the rest is drained.
+//   kCta = 1   M <= 128, bound by reading B: 128 rows x 64 or 128 columns (a tile's scales start at an even TMEM column),
+//              whichever deals N to the SMs; only existing rows of A are loaded.
+//
+// Roles: warp 0 loads A and its scales, warp 6 B and its scales, warp 1 issues, warps 2..5 are the epilogue.
+struct MxGemmParams {
+  CUtensorMap tm_a;   // packed A [M, K / 2 bytes], box (rows per CTA) x 128
+  CUtensorMap tm_b;   // packed B [N, K / 2 bytes], box (width / kCta) x 128
+  CUtensorMap tm_sa;  // scales of A as 8-byte words [row blocks][64 ceil(K / 128)], box 1 x 128
+  CUtensorMap tm_sb;  // scales of B, box 2 x 128
+  CUtensorMap tm_c;   // pair: C [M, N], store box 32 rows x 64 columns
+  void* c;
+  int m, n, k;
+  int width;          // columns per tile
+  int a_rows;         // rows of A that a CTA loads
+  int stages, stage_bytes;
+  int m_tiles, n_tiles, group_m;
+  int bf16;
+  int* status;
+};
+
+template <int kCta>
+struct MxShape {
+  static constexpr int kBK = 256;  // elements of K per stage
+  static constexpr int kABytes = 128 * 128;
+  static constexpr int kScaleBytes = 3 * 1024;
+  static constexpr int kMaxStages = 8;
+  static constexpr int kThreads = 224;
+  static constexpr int kMaxWidth = kCta == 2 ? 256 : 128;
+  static constexpr int kAccStep = kCta == 2 ? 192 : 128;  // TMEM columns from one accumulator to the other
+  static constexpr int kScaleCols = kAccStep + kMaxWidth;  // first column of the scales: two sets of 4 + 8
+  static constexpr int kStagingBytes = kCta == 2 ? 4 * 2 * 4096 : 0;
+  static constexpr int kBarBytes = 256;
+  static constexpr int kSmemLimit = 232448;
+  static constexpr int kRingBytes = kSmemLimit - 1024 - kStagingBytes - kBarBytes;
+  static_assert(kScaleCols + 2 * 12 <= 512, "accumulators and scales share 512 columns");
+  static_assert((2 * kMaxStages + 4) * 8 + 8 <= kBarBytes, "barrier block too small");
+};
+
+template <int kCta>
+__global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(const __grid_constant__ MxGemmParams p) {
+  using S = MxShape<kCta>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t lane = threadIdx.x & 31;
+  const int cta_rank = (kCta == 2) ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+  const bool leader = cta_rank == 0;
+  const int first = static_cast<int>(blockIdx.x) / kCta;
+  const int stride = static_cast<int>(gridDim.x) / kCta;
+  const int tiles = p.m_tiles * p.n_tiles;
+  const int num_kb = (p.k + S::kBK - 1) / S::kBK;
+
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const uint32_t ring_bytes = static_cast<uint32_t>(p.stages * p.stage_bytes);
+  const uint32_t b_bytes = static_cast<uint32_t>(p.width / kCta) * 128u;
+  const uint32_t staging_base = smem_base + ring_bytes;
+  const uint32_t bar_base = staging_base + S::kStagingBytes;
+  auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (S::kMaxStages + s); };
+  auto tmem_full_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + a); };
+  auto tmem_empty_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + 2 + a); };
+  volatile uint32_t* tmem_slot =
+      reinterpret_cast<volatile uint32_t*>(smem_gen + ring_bytes + S::kStagingBytes + 8 * (2 * S::kMaxStages + 4));
+  volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  auto tile_at = [&](int t, int& mt, int& nt) {
+    const int per_group = p.group_m * p.n_tiles;
+    const int g = t / per_group;
+    const int first_m = g * p.group_m;
+    const int rows = min(p.group_m, p.m_tiles - first_m);
+    const int r = t - g * per_group;
+    mt = first_m + r % rows;
+    nt = r / rows;
+  };
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < static_cast<uint32_t>(p.stages); ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (uint32_t a = 0; a < 2; ++a) {
+      ptx::mbar_init(tmem_full_bar(a), 1);
+      ptx::mbar_init(tmem_empty_bar(a), 4 * kCta);
+    }
+    *cta_abort = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&p.tm_a);
+    ptx::prefetch_tensormap(&p.tm_b);
+    ptx::prefetch_tensormap(&p.tm_sa);
+    ptx::prefetch_tensormap(&p.tm_sb);
+    ptx::grid_launch_dependents();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<kCta>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    ptx::tmem_relinquish<kCta>();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (kCta == 2) ptx::cluster_sync_all();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0 || warp == 6) {
+    // ------------------------------------------------------------------ TMA producers
+    if (lane == 0) {
+      ptx::grid_dependency_wait();  // before the first global read
+      const bool left = warp == 0;
+      const uint32_t bytes = static_cast<uint32_t>(kCta) *
+                             (static_cast<uint32_t>(p.a_rows) * 128u + b_bytes + static_cast<uint32_t>(S::kScaleBytes));
+      uint32_t s = 0, ph = 0;
+      bool alive = true;
+      for (int t = first; alive && t < tiles; t += stride) {
+        int mt, nt;
+        tile_at(t, mt, nt);
+        const int block_a = mt * kCta + cta_rank;  // row block of A: 128 rows, one row of scale blocks
+        const int col = nt * p.width;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!bounded_wait(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait)) {
+            alive = false;
+            break;
+          }
+          const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
+          const uint32_t b = a + S::kABytes;
+          const uint32_t sf = b + b_bytes;
+          // A's producer arms the barrier with the whole stage; B's bytes may land before that (see grad_umma.cuh).
+          if (left && leader) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
+          if constexpr (kCta == 2) {
+            const uint32_t bar = ptx::mapa(full_bar(s), 0);
+            if (left) {
+              ptx::tma_load_2d_pair(a, &p.tm_a, bar, kb * 128, block_a * 128);
+              ptx::tma_load_2d_pair(sf, &p.tm_sa, bar, kb * 128, block_a);
+            } else {
+              ptx::tma_load_2d_pair(b, &p.tm_b, bar, kb * 128, col + cta_rank * 128);
+              ptx::tma_load_2d_pair(sf + 1024u, &p.tm_sb, bar, kb * 128, col >> 7);
+            }
+          } else {
+            if (left) {
+              ptx::tma_load_2d(a, &p.tm_a, full_bar(s), kb * 128, block_a * 128);
+              ptx::tma_load_2d(sf, &p.tm_sa, full_bar(s), kb * 128, block_a);
+            } else {
+              ptx::tma_load_2d(b, &p.tm_b, full_bar(s), kb * 128, col);
+              ptx::tma_load_2d(sf + 1024u, &p.tm_sb, full_bar(s), kb * 128, col >> 7);
+            }
+          }
+          if (++s == static_cast<uint32_t>(p.stages)) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0 && leader) {
+      const uint32_t idesc0 = ptx::umma_idesc_mxf4(128 * kCta, p.width, 0);
+      const uint32_t idesc2 = ptx::umma_idesc_mxf4(128 * kCta, p.width, 2);
+      const uint64_t a_desc0 = ptx::umma_desc_k_sw128(smem_base);
+      const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + S::kABytes);
+      const uint64_t sf_desc0 = ptx::umma_desc_scales(smem_base + S::kABytes + b_bytes);
+      const uint64_t desc_stride = static_cast<uint64_t>(p.stage_bytes >> 4);
+      const int steps = (p.k + 63) / 64;  // UMMAs per tile
+      uint32_t s = 0, ph = 0;
+      bool alive = true;
+      for (int t = first, j = 0; alive && t < tiles; t += stride, ++j) {
+        int mt, nt;
+        tile_at(t, mt, nt);
+        const uint32_t acc = static_cast<uint32_t>(j) & 1u;
+        bool drained = true;
+        if constexpr (kCta == 2) {
+          // overlapping accumulators: the previous tile's shared columns must have been read
+          if (j > 0)
+            drained = bounded_wait(tmem_empty_bar(0), static_cast<uint32_t>(j - 1) & 1u, cta_abort, p.status,
+                                   kFaultMmaWaitAcc);
+        } else {
+          drained = bounded_wait(tmem_empty_bar(acc), ((static_cast<uint32_t>(j) >> 1) & 1u) ^ 1u, cta_abort, p.status,
+                                 kFaultMmaWaitAcc);
+        }
+        if (!drained) break;
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * S::kAccStep;
+        // a tile that starts inside a block of 128 columns starts inside that block's four TMEM columns
+        const uint32_t sfb_shift = static_cast<uint32_t>(((nt * p.width) & 127) >> 5);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!bounded_wait(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull)) {
+            alive = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint64_t a = a_desc0 + s * desc_stride, b = b_desc0 + s * desc_stride, sf = sf_desc0 + s * desc_stride;
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) {  // 128 elements of K: one scale block per 128 rows
+            const int step = kb * 4 + static_cast<int>(h) * 2;
+            if (step >= steps) break;
+            const uint32_t sfa = tmem_base + S::kScaleCols + h * 12u, sfb = sfa + 4u;
+            ptx::tmem_cp_scales<kCta>(sfa, sf + h * (512 >> 4));
+            ptx::tmem_cp_scales<kCta>(sfb, sf + ((1024 + h * 512) >> 4));
+            ptx::tmem_cp_scales<kCta>(sfb + 4u, sf + ((2048 + h * 512) >> 4));
+            ptx::umma_mxf4<kCta>(d_tmem, a + h * 4, b + h * 4, idesc0, sfa, sfb + sfb_shift, step > 0 ? 1u : 0u);
+            if (step + 1 < steps)
+              ptx::umma_mxf4<kCta>(d_tmem, a + h * 4 + 2, b + h * 4 + 2, idesc2, sfa, sfb + sfb_shift, 1u);
+          }
+          if constexpr (kCta == 1)
+            ptx::umma_commit<1>(empty_bar(s));
+          else
+            ptx::umma_commit_pair_both(empty_bar(s), 0x3);
+          if (++s == static_cast<uint32_t>(p.stages)) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (alive) {
+          if constexpr (kCta == 1)
+            ptx::umma_commit<1>(tmem_full_bar(acc));
+          else
+            ptx::umma_commit_pair_both(tmem_full_bar(acc), 0x3);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue (warps 2..5)
+    const uint32_t quad = warp & 3u;
+    const uint32_t lead_empty0 = (kCta == 2) ? ptx::mapa(tmem_empty_bar(0), 0) : tmem_empty_bar(0);
+    uint32_t stores = 0;
+    for (int t = first, j = 0; t < tiles; t += stride, ++j) {
+      const uint32_t acc = static_cast<uint32_t>(j) & 1u;
+      const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
+      if (!bounded_wait_warp(tmem_full_bar(acc), acc_ph, cta_abort, p.status, kFaultEpilogueWait, lane)) break;
+      ptx::tc_fence_after();
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int row0 = (mt * kCta + cta_rank) * 128 + static_cast<int>(quad) * 32;
+      const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * S::kAccStep;
+      if constexpr (kCta == 2) {
+        // Columns in chunks of 64, the chunk that the other accumulator shares first: the last of an even tile, the first
+        // of an odd one.
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int c = 64 * (acc == 0 ? (i + 3) & 3 : i);
+          const int col = nt * 256 + c;
+          uint32_t v0[32], v1[32], out[32];
+          ptx::tmem_ld_32x32(taddr + c, v0);
+          ptx::tmem_ld_32x32(taddr + c + 32, v1);
+          ptx::tmem_ld_wait();
+          if (i == 0) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(lead_empty0);
+          }
+          if (row0 >= p.m || col >= p.n) continue;  // warp-uniform
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            out[q] = ptx::pack_out2(__uint_as_float(v0[2 * q]), __uint_as_float(v0[2 * q + 1]), p.bf16);
+            out[16 + q] = ptx::pack_out2(__uint_as_float(v1[2 * q]), __uint_as_float(v1[2 * q + 1]), p.bf16);
+          }
+          const uint32_t buf = staging_base + (quad * 2u + (stores & 1u)) * 4096u;
+          if (stores >= 2) {
+            if (lane == 0) ptx::tma_store_wait_read<1>();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            ptx::st_shared_v4(buf + lane * 128u + ((static_cast<uint32_t>(q) ^ (lane & 7u)) << 4), out[4 * q],
+                              out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]);
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::tma_store_2d(&p.tm_c, buf, col, row0);
+            ptx::tma_store_commit();
+          }
+          ++stores;
+        }
+      } else {
+        const int col0 = nt * p.width;
+        const int row = row0 + static_cast<int>(lane);
+        for (int c = 0; row0 < p.m && c < p.width && col0 + c < p.n; c += 32) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32(taddr + c, v);
+          ptx::tmem_ld_wait();
+          if (row < p.m) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.c) +
+                                                  (static_cast<size_t>(row) * p.n + col0 + c) * 2);
+            const int valid = min(32, p.n - (col0 + c));  // a multiple of 8
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (8 * i < valid) {
+                uint32_t o[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  o[q] = ptx::pack_out2(__uint_as_float(v[8 * i + 2 * q]), __uint_as_float(v[8 * i + 2 * q + 1]), p.bf16);
+                dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+              }
+            }
+          }
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(tmem_empty_bar(acc));
+      }
+    }
+  }
+
+  if (kCta == 2 && warp >= 2 && warp < 6 && lane == 0) ptx::tma_store_wait_read<0>();
+  __syncwarp();
+  if (*cta_abort) abort_drain_delay();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (kCta == 2) ptx::cluster_sync_all();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<kCta>(tmem_base, 512);
+  }
+}
+
+}  // namespace beam

@@ -413,6 +413,22 @@ __device__ __forceinline__ uint64_t umma_desc_k_sw128(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(2) << 61;
   return d;
 }
+// The same for an operand whose contraction runs over the ROWS of memory (M- or N-major): a TMA box of 64 elements x 64
+// rows of the contraction is 64 rows of 128 bytes, 8-row groups 1024 bytes apart; the next 64 elements of M or N are the
+// next box, 8192 bytes further.
+//   [16,30) leading byte offset: from one 64-element run of M or N to the next   [32,46) stride byte offset: 8 steps of K
+// A UMMA's 16 steps of K are two 8-row groups: the start address advances by 2048 bytes.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(8192 >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+constexpr uint32_t kIdescAMnMajor = 1u << 15;  // OR into the instruction descriptor
+constexpr uint32_t kIdescBMnMajor = 1u << 16;
 // Instruction descriptor, kind::f16: fp16 A and B, both K-major, fp32 D, shape M x N.
 //   [4,6) D format 1=f32   [7,10) A format 0=f16, 1=bf16   [10,13) B format 0=f16, 1=bf16
 //   [15] A major 0=K   [16] B major 0=K   [17,23) N>>3   [24,29) M>>4
@@ -430,10 +446,102 @@ __device__ __forceinline__ uint32_t pack_out2(float lo, float hi, int bf16) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+// The two 16-bit values of a word as fp32.
+__device__ __forceinline__ float2 unpack_in2(uint32_t v, int bf16) {
+  if (bf16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
 constexpr uint32_t kIdescBf16Inputs = (1u << 7) | (1u << 10);  // OR into the descriptor for bf16 A and B
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
+}
+
+
+// ------------------------------------------------------------------ 4-bit operands with block scales
+// D (+)= (SFA A) (SFB B): e2m1 operands in shared memory, one ue8m0 scale per 32 elements of K in TMEM (scale_vec::2X: a
+// K = 64 step takes two scales per row; the instruction descriptor says which two of a column's four bytes).
+template <int kCta>
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  if constexpr (kCta == 1)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor, kind::mxf4, dense, K = 64, D fp32, both operands K-major.
+//   [4,6) byte of B's scales   [7,10) A format 1 = e2m1   [10,13) B format   [17,23) N>>3   [23] scales 1 = ue8m0
+//   [24,29) M>>4   [29,31) byte of A's scales
+__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int m, int n, int scale_byte) {
+  return (static_cast<uint32_t>(scale_byte) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) | (static_cast<uint32_t>(scale_byte) << 29);
+}
+// Copies 32 rows x 16 bytes (512 contiguous bytes of shared memory) into 4 columns of 32 TMEM lanes, repeated in each of
+// the four lane quarters: how a block of 128 rows x 4 scales is handed to umma_mxf4.  On a pair one thread issues the
+// copy for both CTAs, each from its own shared memory.  Executes in order with the UMMAs this thread issues.
+template <int kCta>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (kCta == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Descriptor of such a block: no swizzle, 8-row groups of 16-byte rows are 128 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_scales(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+// Eight fp32 values to e2m1, nearest even, saturating at 6; element i in bits [4 i, 4 i + 4).
+__device__ __forceinline__ uint32_t pack_e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t"
+      ".reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t"
+      "}\n"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// ... and back: element pairs as fp16, exactly.
+__device__ __forceinline__ void unpack_e2m1x8(uint32_t q, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t"
+      ".reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t"
+      "}\n"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(q));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
 }
 
 }  // namespace ptx

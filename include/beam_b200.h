@@ -230,6 +230,68 @@ BEAM_API int beam_gemmrc_layernorm(const void* X, const void* W, void* out, cons
 BEAM_API int beam_gemmrc_silu(const void* A, const void* B, void* C, int m, int n, int k, const void* x, void* y,
                               long long count, void* stream);
 
+/* ---- feed-forward block: gated product and gradients ---------------------------------------------- */
+
+/* Activations of the gated product, g the gate's projection: */
+#define BEAM_ACT_SILU 0      /* g / (1 + exp(-g)) */
+#define BEAM_ACT_GELU 1      /* g (1 + erf(g / sqrt 2)) / 2 */
+#define BEAM_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+#define BEAM_ACT_RELU 3      /* max(g, 0); its slope at 0 is 0 */
+
+/* C[M,F] = act(G) * U with G = A x B_gate^T and U = A x B_up^T: both products, the activation and their element-wise
+ * product in one kernel (no counterpart in the reference).  A [M,K], B_gate and B_up [F,K], all fp16, or all bf16 with
+ * BEAM_FLAG_BF16 (the only flag).  fp32 accumulation; G and U are combined in fp32 and C is rounded once.
+ * gate, up: both NULL, or both [M,F] outputs that keep G and U (each rounded once) for the backward pass.
+ * K % 8 == 0, F % 8 == 0, any M; outputs overlap neither the inputs nor each other. */
+BEAM_API int beam_gated_gemmrc(const void* A, const void* B_gate, const void* B_up, void* C, void* gate, void* up, int m,
+                               int f, int k, int activation, int flags, void* stream);
+
+/* Scratch bytes for beam_gated_gemmrc_backward: dG and dU. */
+BEAM_API size_t beam_gated_gemmrc_backward_workspace_bytes(int m, int f, int k);
+
+/* Gradients of beam_gated_gemmrc, given dC [M,F] and the kept gate and up:
+ *   dG = dC * up * act'(gate), dU = dC * act(gate)      (fp32, rounded once to the operands' type, in `workspace`)
+ *   dA = dG x B_gate + dU x B_up,  dB_gate = dG^T x A,  dB_up = dU^T x A      (fp32 accumulation, one rounding)
+ * Any of dA, dB_gate and dB_up may be NULL, but not all three; B_gate and B_up may be NULL without dA, and A without dB_gate and
+ * dB_up.  Outputs are overwritten (no accumulation into them), and overlap neither the inputs nor each other nor the workspace. */
+BEAM_API int beam_gated_gemmrc_backward(const void* dC, const void* A, const void* B_gate, const void* B_up,
+                                        const void* gate, const void* up, void* dA, void* dB_gate, void* dB_up, int m,
+                                        int f, int k, int activation, int flags, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+
+/* Gradients of the rc GEMM C = A x B^T: dA[M,K] = dC[M,N] x B[N,K] and dB[N,K] = dC^T x A[M,K], in one launch, without
+ * transposing anything in memory.  fp16, or bf16 with BEAM_FLAG_BF16.  dA or dB may be NULL (then B, or A, may be too). */
+BEAM_API int beam_gemmrc_backward(const void* dC, const void* A, const void* B, void* dA, void* dB, int m, int n, int k,
+                                  int flags, void* stream);
+
+/* ---- MXFP4: microscaled 4-bit floating point ------------------------------------------------------- */
+
+/* A quantised matrix [rows, K], K % 32 == 0, is
+ *   q       [rows, K / 2] bytes: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), element 2 i in the low half
+ *           of byte i;
+ *   scales  one byte s per 32 elements of a row, worth 2^(s - 127) (255: NaN), in blocks of 128 rows x 4 scales:
+ *           [ceil(rows / 128)][ceil(K / 128)][512], row r and scale c of a block at byte (r % 32) * 16 + (r / 32) * 4 + c.
+ *           Bytes outside the matrix are 0 (beam_mxfp4_quantize writes them; beam_mxfp4_gemmrc relies on those past K). */
+#define BEAM_TYPE_FP16 0
+#define BEAM_TYPE_BF16 1
+#define BEAM_TYPE_FP32 2
+
+/* Bytes of the scales of a [rows, K] matrix, padding included. */
+BEAM_API size_t beam_mxfp4_scales_bytes(int rows, int k);
+
+/* x [rows, K] fp16 (bf16 with BEAM_FLAG_BF16) -> q, scales.  The scale is 2 to the power floor(log2(max |x|)) - 2 of its 32
+ * elements, at least 2^-127; elements are divided by it and rounded to the nearest code, ties to even codes, magnitudes
+ * above 6 to 6.  A block that holds an infinity or a NaN becomes NaN as a whole. */
+BEAM_API int beam_mxfp4_quantize(const void* x, void* q, void* scales, int rows, int k, int flags, void* stream);
+
+/* The values of a quantised matrix as x [rows, K] of `type` (BEAM_TYPE_*), each rounded once (exact in bf16 and fp32). */
+BEAM_API int beam_mxfp4_dequantize(const void* q, const void* scales, void* x, int rows, int k, int type, void* stream);
+
+/* C[M,N] = A x B^T of two quantised matrices A [M,K] and B [N,K] on the 4-bit tensor cores: fp32 accumulation, one rounding
+ * to fp16 (bf16 with BEAM_FLAG_BF16).  N % 8 == 0, K % 32 == 0. */
+BEAM_API int beam_mxfp4_gemmrc(const void* A, const void* a_scales, const void* B, const void* b_scales, void* C, int m,
+                               int n, int k, int flags, void* stream);
+
 /* ---- host-buffer convenience (what a caller with pageable or pinned HOST arrays uses) ---------- */
 
 /* A, B, C are HOST pointers (pinned memory for full PCIe speed).  A and B go to the device in alternating row
