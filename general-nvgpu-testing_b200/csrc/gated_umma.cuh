@@ -47,7 +47,8 @@ struct GatedShape {
   static constexpr int kBK = 64;
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kMaxStages = 8;
-  static constexpr int kThreads = 192;
+  static constexpr int kProducers = kCta == 1 ? 4 : 2;
+  static constexpr int kThreads = 32 * (5 + kProducers);
   static constexpr int kAccCols = 256;  // TMEM columns between the two accumulators
   static constexpr int kBufsPerWarp = 4;
   static constexpr int kStoreBufBytes = 32 * 64;
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
     gated_umma_kernel(const __grid_constant__ GatedParams p) {
   using S = GatedShape<kCta>;
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t warp = ptx::warp_index();
   const uint32_t lane = threadIdx.x & 31;
   const uint32_t cta_rank = (kCta == 2) ? ptx::cluster_ctarank() : 0u;
   const bool leader = cta_rank == 0;
@@ -137,82 +138,91 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      ptx::grid_dependency_wait();  // before the first global read; everything else follows from these reads
-      const uint32_t b_bytes = static_cast<uint32_t>(p.width) * 128u;
-      const uint32_t bytes = 2u * b_bytes + static_cast<uint32_t>(kCta) * static_cast<uint32_t>(p.a_rows) * 128u;
-      uint32_t s = 0, ph = 0;
-      bool alive = true;
-      for (int t = first; alive && t < tiles; t += stride) {
-        int mt, nt;
-        tile_at(t, mt, nt);
-        const int row_a = (mt * kCta + static_cast<int>(cta_rank)) * S::kBM;
-        const int row_b = nt * p.width;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait)) {
-            alive = false;
-            break;
-          }
+  if (warp == 0 || warp >= 6) {
+    // ------------------------------------------------------------------ TMA producers
+    ptx::grid_dependency_wait();  // before the first global read; everything else follows from these reads
+    const uint32_t b_bytes = static_cast<uint32_t>(p.width) * 128u;
+    const uint32_t bytes = 2u * b_bytes + static_cast<uint32_t>(kCta) * static_cast<uint32_t>(p.a_rows) * 128u;
+    const uint32_t mine = warp == 0 ? 0u : warp - 5u;  // this warp fills every kProducers-th stage of the walk
+    const uint32_t stages = static_cast<uint32_t>(p.stages);
+    const CUtensorMap* tm_b = leader ? &p.tm_gate : &p.tm_up;
+    uint32_t s = mine % stages, ph = (mine / stages) & 1u;
+    int kb = static_cast<int>(mine);
+    for (int t = first; t < tiles; t += stride) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int row_a = (mt * kCta + static_cast<int>(cta_rank)) * S::kBM;
+      const int row_b = nt * p.width;
+      for (; kb < num_kb; kb += S::kProducers) {
+        if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) break;
+        if (ptx::elect_one()) {
           const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
           const uint32_t b = a + S::kABytes;
           if (leader) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
           if constexpr (kCta == 2) {
             const uint32_t bar = ptx::mapa(full_bar(s), 0);
             ptx::tma_load_2d_pair(a, &p.tm_a, bar, kb * S::kBK, row_a);
-            ptx::tma_load_2d_pair(b, leader ? &p.tm_gate : &p.tm_up, bar, kb * S::kBK, row_b);
+            ptx::tma_load_2d_pair(b, tm_b, bar, kb * S::kBK, row_b);
           } else {
             ptx::tma_load_2d(b, &p.tm_gate, full_bar(s), kb * S::kBK, row_b);
             ptx::tma_load_2d(b + b_bytes, &p.tm_up, full_bar(s), kb * S::kBK, row_b);
             ptx::tma_load_2d(a, &p.tm_a, full_bar(s), kb * S::kBK, row_a);
           }
-          if (++s == static_cast<uint32_t>(p.stages)) {
-            s = 0;
-            ph ^= 1u;
-          }
+        }
+        __syncwarp();
+        s += S::kProducers;
+        while (s >= stages) {
+          s -= stages;
+          ph ^= 1u;
         }
       }
+      if (kb < num_kb) break;  // a wait ran out
+      kb -= num_kb;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && leader) {
+    if (leader) {
       const uint32_t idesc =
           ptx::umma_idesc_f16_f32(S::kBM * kCta, 2 * p.width) | (p.bf16 ? ptx::kIdescBf16Inputs : 0u);
       const uint64_t a_desc0 = ptx::umma_desc_k_sw128(smem_base);
       const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + S::kABytes);
       const uint64_t desc_stride = static_cast<uint64_t>(p.stage_bytes >> 4);
+      const uint32_t stages = static_cast<uint32_t>(p.stages);
       uint32_t s = 0, ph = 0;
       bool alive = true;
       for (int t = first, j = 0; alive && t < tiles; t += stride, ++j) {
         const uint32_t acc = static_cast<uint32_t>(j) & 1u;
         const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
-        if (!bounded_wait(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc)) break;
+        if (!bounded_wait_converged(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc, lane)) break;
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * S::kAccCols;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull)) {
+          if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) {
             alive = false;
             break;
           }
           ptx::tc_fence_after();
-          ptx::umma_f16_kblock<kCta>(d_tmem, a_desc0 + s * desc_stride, b_desc0 + s * desc_stride, idesc,
-                                     kb > 0 ? 1u : 0u);
-          if constexpr (kCta == 1)
-            ptx::umma_commit<1>(empty_bar(s));
-          else
-            ptx::umma_commit_pair_both(empty_bar(s), 0x3);
-          if (++s == static_cast<uint32_t>(p.stages)) {
+          if (ptx::elect_one()) {
+            ptx::umma_f16_kblock<kCta>(d_tmem, a_desc0 + s * desc_stride, b_desc0 + s * desc_stride, idesc,
+                                       kb > 0 ? 1u : 0u);
+            if constexpr (kCta == 1)
+              ptx::umma_commit<1>(empty_bar(s));
+            else
+              ptx::umma_commit_pair_both(empty_bar(s), 0x3);
+          }
+          __syncwarp();
+          if (++s == stages) {
             s = 0;
             ph ^= 1u;
           }
         }
-        if (alive) {
+        if (alive && ptx::elect_one()) {
           if constexpr (kCta == 1)
             ptx::umma_commit<1>(tmem_full_bar(acc));
           else
             ptx::umma_commit_pair_both(tmem_full_bar(acc), 0x3);
         }
+        __syncwarp();
       }
     }
   } else {
@@ -294,7 +304,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
   }
 
   // ---- teardown: bulk stores have read their staging buffers; then everyone meets and the allocating warp frees TMEM
-  if (kCta == 2 && warp >= 2 && lane == 0) ptx::tma_store_wait_read<0>();
+  if (kCta == 2 && warp >= 2 && warp < 6 && lane == 0) ptx::tma_store_wait_read<0>();
   __syncwarp();
   if (*cta_abort) abort_drain_delay();
   ptx::tc_fence_before();

@@ -76,7 +76,7 @@ __device__ __forceinline__ const GradJob& grad_tile(const GradParams& p, int t, 
 static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kernel(const __grid_constant__ GradParams p) {
   using S = GradShape;
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t warp = ptx::warp_index();
   const uint32_t lane = threadIdx.x & 31;
   const int cta_rank = static_cast<int>(ptx::cluster_ctarank());
   const bool leader = cta_rank == 0;
@@ -120,24 +120,24 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
 
   if (warp == 0 || warp == 6) {
     // ------------------------------------------------------------------ TMA producers
-    if (lane == 0) {
-      ptx::grid_dependency_wait();  // before the first global read
-      const bool left = warp == 0;
-      uint32_t s = 0, ph = 0;
-      bool alive = true;
-      for (int t = first; alive && t < p.tiles; t += stride) {
-        int mt, nt;
-        const GradJob& job = grad_tile(p, t, mt, nt);
-        const int row = mt * 256 + cta_rank * 128;
-        const int col = nt * 256 + cta_rank * 128;
-        const int num_kb = (job.contraction + S::kBK - 1) / S::kBK;
-        for (int seg = 0; alive && seg < job.segments; ++seg) {
-          const CUtensorMap* map = left ? &job.tm_a[seg] : &job.tm_b[seg];
-          for (int kb = 0; kb < num_kb; ++kb) {
-            if (!bounded_wait(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait)) {
-              alive = false;
-              break;
-            }
+    ptx::grid_dependency_wait();  // before the first global read
+    const bool left = warp == 0;
+    uint32_t s = 0, ph = 0;
+    bool alive = true;
+    for (int t = first; alive && t < p.tiles; t += stride) {
+      int mt, nt;
+      const GradJob& job = grad_tile(p, t, mt, nt);
+      const int row = mt * 256 + cta_rank * 128;
+      const int col = nt * 256 + cta_rank * 128;
+      const int num_kb = (job.contraction + S::kBK - 1) / S::kBK;
+      for (int seg = 0; alive && seg < job.segments; ++seg) {
+        const CUtensorMap* map = left ? &job.tm_a[seg] : &job.tm_b[seg];
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) {
+            alive = false;
+            break;
+          }
+          if (ptx::elect_one()) {
             // The left producer of the leader arms the barrier with all bytes of both CTAs; bytes of the right operand
             // that land before that only make the pending count negative for a moment, the phase still needs the arrive.
             if (left && leader) ptx::mbar_arrive_expect_tx(full_bar(s), 2u * S::kStageBytes);
@@ -151,17 +151,18 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
               ptx::tma_load_2d_pair(dst, map, bar, along, kb * S::kBK);
               ptx::tma_load_2d_pair(dst + 8192u, map, bar, along + 64, kb * S::kBK);
             }
-            if (++s == S::kStages) {
-              s = 0;
-              ph ^= 1u;
-            }
+          }
+          __syncwarp();
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1u;
           }
         }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && leader) {
+    if (leader) {
       const uint32_t idesc0 = ptx::umma_idesc_f16_f32(256, 256) | ptx::kIdescBMnMajor |
                               (p.bf16 ? ptx::kIdescBf16Inputs : 0u);
       const uint64_t a_desc_k = ptx::umma_desc_k_sw128(smem_base);
@@ -175,7 +176,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
         const GradJob& job = grad_tile(p, t, mt, nt);
         const uint32_t acc = static_cast<uint32_t>(j) & 1u;
         const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
-        if (!bounded_wait(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc)) break;
+        if (!bounded_wait_converged(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc, lane)) break;
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256u;
         const uint32_t idesc = idesc0 | (job.a_mn ? ptx::kIdescAMnMajor : 0u);
@@ -183,22 +184,26 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
         const uint64_t a_step = job.a_mn ? (2048 >> 4) : (32 >> 4);  // 16 steps of the contraction
         const int num_kb = (job.contraction + S::kBK - 1) / S::kBK * job.segments;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull)) {
+          if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) {
             alive = false;
             break;
           }
           ptx::tc_fence_after();
-          const uint64_t a = a_desc0 + s * kDescStride, b = b_desc0 + s * kDescStride;
+          if (ptx::elect_one()) {
+            const uint64_t a = a_desc0 + s * kDescStride, b = b_desc0 + s * kDescStride;
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i)
-            ptx::umma_f16<2>(d_tmem, a + i * a_step, b + i * (2048 >> 4), idesc, (kb > 0 || i > 0) ? 1u : 0u);
-          ptx::umma_commit_pair_both(empty_bar(s), 0x3);
+            for (uint32_t i = 0; i < 4; ++i)
+              ptx::umma_f16<2>(d_tmem, a + i * a_step, b + i * (2048 >> 4), idesc, (kb > 0 || i > 0) ? 1u : 0u);
+            ptx::umma_commit_pair_both(empty_bar(s), 0x3);
+          }
+          __syncwarp();
           if (++s == S::kStages) {
             s = 0;
             ph ^= 1u;
           }
         }
-        if (alive) ptx::umma_commit_pair_both(tmem_full_bar(acc), 0x3);
+        if (alive && ptx::elect_one()) ptx::umma_commit_pair_both(tmem_full_bar(acc), 0x3);
+        __syncwarp();
       }
     }
   } else {

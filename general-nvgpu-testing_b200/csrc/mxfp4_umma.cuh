@@ -136,9 +136,9 @@ static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint
 // C[M, N] = A B^T: 4-bit UMMAs (K = 64) with block scales, fp32 accumulation, one rounding to fp16 or bf16.
 //
 // A stage of the ring is 256 elements of K: 128 bytes per row, laid out by TMA with the 128-byte swizzle like any K-major
-// operand, and 3 KB of scale blocks (one row block for A, two for B) that a second copy brings as they are.  Per 128
-// elements the issuing thread copies three scale blocks into TMEM and issues two UMMAs; copies and UMMAs of one thread
-// execute in order, so nothing else separates them; two sets of scale columns alternate.
+// operand, and 3 KB of scale blocks (one row block for A, two for B) that a second copy brings as they are.  Per stage
+// the issuing thread copies six scale blocks into TMEM and issues four UMMAs; copies and UMMAs of one thread execute in
+// order, so nothing else separates them; two sets of scale columns alternate.
 //
 //   kCta = 2   256 x 256 tiles on a pair.  B's scales of all 256 columns are needed in both CTAs' TMEM, so both load them.
 //              Two accumulators of 256 columns and the scales do not fit into 512 columns, so the accumulators overlap
@@ -173,12 +173,12 @@ struct MxShape {
   static constexpr int kThreads = 224;
   static constexpr int kMaxWidth = kCta == 2 ? 256 : 128;
   static constexpr int kAccStep = kCta == 2 ? 192 : 128;  // TMEM columns from one accumulator to the other
-  static constexpr int kScaleCols = kAccStep + kMaxWidth;  // first column of the scales: two sets of 4 + 8
+  static constexpr int kScaleCols = kAccStep + kMaxWidth;  // first column of the scales: two sets of 2 x (4 + 8)
   static constexpr int kStagingBytes = kCta == 2 ? 4 * 2 * 4096 : 0;
   static constexpr int kBarBytes = 256;
   static constexpr int kSmemLimit = 232448;
   static constexpr int kRingBytes = kSmemLimit - 1024 - kStagingBytes - kBarBytes;
-  static_assert(kScaleCols + 2 * 12 <= 512, "accumulators and scales share 512 columns");
+  static_assert(kScaleCols + 2 * 24 <= 512, "accumulators and scales share 512 columns");
   static_assert((2 * kMaxStages + 4) * 8 + 8 <= kBarBytes, "barrier block too small");
 };
 
@@ -186,7 +186,7 @@ template <int kCta>
 __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(const __grid_constant__ MxGemmParams p) {
   using S = MxShape<kCta>;
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t warp = ptx::warp_index();
   const uint32_t lane = threadIdx.x & 31;
   const int cta_rank = (kCta == 2) ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   const bool leader = cta_rank == 0;
@@ -248,23 +248,24 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
 
   if (warp == 0 || warp == 6) {
     // ------------------------------------------------------------------ TMA producers
-    if (lane == 0) {
-      ptx::grid_dependency_wait();  // before the first global read
-      const bool left = warp == 0;
-      const uint32_t bytes = static_cast<uint32_t>(kCta) *
-                             (static_cast<uint32_t>(p.a_rows) * 128u + b_bytes + static_cast<uint32_t>(S::kScaleBytes));
-      uint32_t s = 0, ph = 0;
-      bool alive = true;
-      for (int t = first; alive && t < tiles; t += stride) {
-        int mt, nt;
-        tile_at(t, mt, nt);
-        const int block_a = mt * kCta + cta_rank;  // row block of A: 128 rows, one row of scale blocks
-        const int col = nt * p.width;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait)) {
-            alive = false;
-            break;
-          }
+    ptx::grid_dependency_wait();  // before the first global read
+    const bool left = warp == 0;
+    const uint32_t bytes = static_cast<uint32_t>(kCta) *
+                           (static_cast<uint32_t>(p.a_rows) * 128u + b_bytes + static_cast<uint32_t>(S::kScaleBytes));
+    const uint32_t stages = static_cast<uint32_t>(p.stages);
+    uint32_t s = 0, ph = 0;
+    bool alive = true;
+    for (int t = first; alive && t < tiles; t += stride) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int block_a = mt * kCta + cta_rank;  // row block of A: 128 rows, one row of scale blocks
+      const int col = nt * p.width;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) {
+          alive = false;
+          break;
+        }
+        if (ptx::elect_one()) {
           const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
           const uint32_t b = a + S::kABytes;
           const uint32_t sf = b + b_bytes;
@@ -288,24 +289,28 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
               ptx::tma_load_2d(sf + 1024u, &p.tm_sb, full_bar(s), kb * 128, col >> 7);
             }
           }
-          if (++s == static_cast<uint32_t>(p.stages)) {
-            s = 0;
-            ph ^= 1u;
-          }
+        }
+        __syncwarp();
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
         }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && leader) {
+    if (leader) {
       const uint32_t idesc0 = ptx::umma_idesc_mxf4(128 * kCta, p.width, 0);
       const uint32_t idesc2 = ptx::umma_idesc_mxf4(128 * kCta, p.width, 2);
       const uint64_t a_desc0 = ptx::umma_desc_k_sw128(smem_base);
       const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + S::kABytes);
       const uint64_t sf_desc0 = ptx::umma_desc_scales(smem_base + S::kABytes + b_bytes);
       const uint64_t desc_stride = static_cast<uint64_t>(p.stage_bytes >> 4);
+      const uint32_t stages = static_cast<uint32_t>(p.stages);
       const int steps = (p.k + 63) / 64;  // UMMAs per tile
-      uint32_t s = 0, ph = 0;
+      const uint32_t scale_cols = tmem_base + S::kScaleCols;
+
+      uint32_t s = 0, ph = 0, set = 0;
       bool alive = true;
       for (int t = first, j = 0; alive && t < tiles; t += stride, ++j) {
         int mt, nt;
@@ -315,11 +320,11 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         if constexpr (kCta == 2) {
           // overlapping accumulators: the previous tile's shared columns must have been read
           if (j > 0)
-            drained = bounded_wait(tmem_empty_bar(0), static_cast<uint32_t>(j - 1) & 1u, cta_abort, p.status,
-                                   kFaultMmaWaitAcc);
+            drained = bounded_wait_converged(tmem_empty_bar(0), static_cast<uint32_t>(j - 1) & 1u, cta_abort, p.status,
+                                             kFaultMmaWaitAcc, lane);
         } else {
-          drained = bounded_wait(tmem_empty_bar(acc), ((static_cast<uint32_t>(j) >> 1) & 1u) ^ 1u, cta_abort, p.status,
-                                 kFaultMmaWaitAcc);
+          drained = bounded_wait_converged(tmem_empty_bar(acc), ((static_cast<uint32_t>(j) >> 1) & 1u) ^ 1u, cta_abort,
+                                           p.status, kFaultMmaWaitAcc, lane);
         }
         if (!drained) break;
         ptx::tc_fence_after();
@@ -327,39 +332,45 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         // a tile that starts inside a block of 128 columns starts inside that block's four TMEM columns
         const uint32_t sfb_shift = static_cast<uint32_t>(((nt * p.width) & 127) >> 5);
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull)) {
+          if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) {
             alive = false;
             break;
           }
           ptx::tc_fence_after();
-          const uint64_t a = a_desc0 + s * desc_stride, b = b_desc0 + s * desc_stride, sf = sf_desc0 + s * desc_stride;
+          if (ptx::elect_one()) {
+            const uint64_t a = a_desc0 + s * desc_stride, b = b_desc0 + s * desc_stride, sf = sf_desc0 + s * desc_stride;
+            const uint32_t sfa = scale_cols + set * 24u, sfb = sfa + 4u;
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {  // 128 elements of K: one scale block per 128 rows
-            const int step = kb * 4 + static_cast<int>(h) * 2;
-            if (step >= steps) break;
-            const uint32_t sfa = tmem_base + S::kScaleCols + h * 12u, sfb = sfa + 4u;
-            ptx::tmem_cp_scales<kCta>(sfa, sf + h * (512 >> 4));
-            ptx::tmem_cp_scales<kCta>(sfb, sf + ((1024 + h * 512) >> 4));
-            ptx::tmem_cp_scales<kCta>(sfb + 4u, sf + ((2048 + h * 512) >> 4));
-            ptx::umma_mxf4<kCta>(d_tmem, a + h * 4, b + h * 4, idesc0, sfa, sfb + sfb_shift, step > 0 ? 1u : 0u);
-            if (step + 1 < steps)
-              ptx::umma_mxf4<kCta>(d_tmem, a + h * 4 + 2, b + h * 4 + 2, idesc2, sfa, sfb + sfb_shift, 1u);
+            for (uint32_t h = 0; h < 2; ++h) {
+              ptx::tmem_cp_scales<kCta>(sfa + h * 12u, sf + h * (512 >> 4));
+              ptx::tmem_cp_scales<kCta>(sfb + h * 12u, sf + ((1024 + h * 512) >> 4));
+              ptx::tmem_cp_scales<kCta>(sfb + h * 12u + 4u, sf + ((2048 + h * 512) >> 4));
+            }
+            const int live = steps - kb * 4;  // steps past K are left out: their scales may lie outside the matrix
+            const uint32_t from = sfb + sfb_shift;
+            ptx::umma_mxf4<kCta>(d_tmem, a, b, idesc0, sfa, from, kb > 0 ? 1u : 0u);
+            if (live > 1) ptx::umma_mxf4<kCta>(d_tmem, a + 2, b + 2, idesc2, sfa, from, 1u);
+            if (live > 2) ptx::umma_mxf4<kCta>(d_tmem, a + 4, b + 4, idesc0, sfa + 12u, from + 12u, 1u);
+            if (live > 3) ptx::umma_mxf4<kCta>(d_tmem, a + 6, b + 6, idesc2, sfa + 12u, from + 12u, 1u);
+            if constexpr (kCta == 1)
+              ptx::umma_commit<1>(empty_bar(s));
+            else
+              ptx::umma_commit_pair_both(empty_bar(s), 0x3);
           }
-          if constexpr (kCta == 1)
-            ptx::umma_commit<1>(empty_bar(s));
-          else
-            ptx::umma_commit_pair_both(empty_bar(s), 0x3);
-          if (++s == static_cast<uint32_t>(p.stages)) {
+          __syncwarp();
+          set ^= 1u;
+          if (++s == stages) {
             s = 0;
             ph ^= 1u;
           }
         }
-        if (alive) {
+        if (alive && ptx::elect_one()) {
           if constexpr (kCta == 1)
             ptx::umma_commit<1>(tmem_full_bar(acc));
           else
             ptx::umma_commit_pair_both(tmem_full_bar(acc), 0x3);
         }
+        __syncwarp();
       }
     }
   } else {

@@ -21,6 +21,23 @@ __device__ __forceinline__ uint32_t lane_id() {
   return v;
 }
 
+// The warp's index, known to the compiler as the same in all its lanes, and one lane of a converged warp.  A role that issues
+// tcgen05 or TMA instructions in a loop runs that loop in the whole warp and only issues under elect_one(): descriptors,
+// addresses and loop counters then live in uniform registers, which those instructions take their operands from.  Inside a branch
+// on lane 0 every operand is moved there anew: 590 cycles per 64-wide k-block in the issuing thread of the gated product, of
+// which 270 for four UMMAs, against the 512 that the tensor pipe needs for a 256 x 256 tile's.
+__device__ __forceinline__ uint32_t warp_index() { return __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ uint64_t globaltimer_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));

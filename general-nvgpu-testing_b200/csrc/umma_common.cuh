@@ -81,6 +81,17 @@ __device__ __forceinline__ bool bounded_wait_warp(uint32_t bar, uint32_t parity,
   return ok != 0;
 }
 
+// The same wait for warps that run their loop converged (see ptx::elect_one): every lane tests once, and when the phase is not
+// complete yet lane 0 waits for all.  Returns the same value in every lane.
+__device__ __forceinline__ bool bounded_wait_converged(uint32_t bar, uint32_t parity, volatile int* cta_abort,
+                                                       int* status_word, int fault, uint32_t lane) {
+  const bool hit = ptx::mbar_try_wait(bar, parity);
+  if (__all_sync(0xffffffffu, hit)) return true;
+  const bool ok = bounded_wait_warp(bar, parity, cta_abort, status_word, fault, lane);
+  __syncwarp();
+  return ok;
+}
+
 // After an abort, give asynchronous work this CTA already issued (TMA copies into its shared
 // memory, UMMAs into its TMEM) time to land before shared memory and TMEM are released.
 __device__ __forceinline__ void abort_drain_delay() {
