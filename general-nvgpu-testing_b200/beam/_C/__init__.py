@@ -378,6 +378,9 @@ _HALF_TYPES = (torch.float16, torch.bfloat16)
 def _check_matrix(name, t, shape, dtype, device):
     """A contiguous CUDA tensor of this shape, type and device; shape or device None: any of two dimensions, any CUDA device;
     dtype may be a tuple of choices."""
+    if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.device == device
+            and t.is_contiguous()):
+        return  # the usual case, by few tests: a call's host time is of the order of a small kernel's
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor" % name)
     if t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
@@ -390,6 +393,17 @@ def _check_matrix(name, t, shape, dtype, device):
         raise ValueError("%s must be %s, got %s" % (name, "2-D" if shape is None else tuple(shape), tuple(t.shape)))
     if device is not None and t.device != device:
         raise ValueError("%s must be on %s, like the other tensors" % (name, device))
+
+
+def _check_first(name, t, dtypes):
+    """The tensor that says type, device and sizes: 2-D, contiguous, on a CUDA device.  Returns its two sizes."""
+    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.is_cuda and t.dim() == 2 and t.is_contiguous()):
+        _check_matrix(name, t, None, dtypes, None)
+    return t.shape
+
+
+def _rows(t):
+    return t.shape[0] if isinstance(t, torch.Tensor) and t.dim() == 2 else -1
 
 
 def _activation(name):
@@ -406,11 +420,20 @@ def _half_flags(t):
     return 2 if t.dtype == torch.bfloat16 else 0
 
 
+# The current stream's handle of a device, without building a torch.cuda.Stream (2 us a call) where torch offers that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(fn_name, device, *args):
     """Calls a C entry with `device` current, on torch's current stream of that device (its last argument)."""
-    L = _load()
-    with torch.cuda.device(device):
-        st = getattr(L, fn_name)(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    fn = getattr(_lib or _load(), fn_name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        st = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, _raw_stream(index))
     if st != BEAM_OK:
         _raise(st, fn_name)
 
@@ -422,19 +445,17 @@ def gated_gemmrc(a, b_gate, b_up, c, activation="silu", gate=None, up=None):
     (the erf form), "gelu_tanh" or "relu".  The products are accumulated and combined in fp32 and c is rounded once.
     gate and up, given together, are [M,F] outputs that keep the two products for gated_gemmrc_backward."""
     act = _activation(activation)
-    _check_matrix("a", a, None, _HALF_TYPES, None)
-    m, k = a.shape
-    _check_matrix("b_gate", b_gate, None, a.dtype, a.device)
-    f = b_gate.shape[0]
-    _check_matrix("b_gate", b_gate, (f, k), a.dtype, a.device)
-    _check_matrix("b_up", b_up, (f, k), a.dtype, a.device)
-    _check_matrix("c", c, (m, f), a.dtype, a.device)
+    m, k = _check_first("a", a, _HALF_TYPES)
+    dtype, device, f = a.dtype, a.device, _rows(b_gate)
+    _check_matrix("b_gate", b_gate, (f, k), dtype, device)
+    _check_matrix("b_up", b_up, (f, k), dtype, device)
+    _check_matrix("c", c, (m, f), dtype, device)
     if (gate is None) != (up is None):
         raise ValueError("gate and up must be given together")
     if gate is not None:
-        _check_matrix("gate", gate, (m, f), a.dtype, a.device)
-        _check_matrix("up", up, (m, f), a.dtype, a.device)
-    _call("beam_gated_gemmrc", a.device, a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(), c.data_ptr(), _ptr(gate),
+        _check_matrix("gate", gate, (m, f), dtype, device)
+        _check_matrix("up", up, (m, f), dtype, device)
+    _call("beam_gated_gemmrc", device, a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(), c.data_ptr(), _ptr(gate),
           _ptr(up), m, f, k, act, _half_flags(a))
 
 
@@ -447,21 +468,24 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
     (at least one) and overwritten.  dg and du are rounded to the operands' type between the two steps; they are
     held in scratch of 4 M F bytes from torch's allocator."""
     act = _activation(activation)
-    _check_matrix("a", a, None, _HALF_TYPES, None)
-    m, k = a.shape
-    _check_matrix("b_gate", b_gate, None, a.dtype, a.device)
-    f = b_gate.shape[0]
-    wanted = [("b_gate", b_gate, (f, k)), ("b_up", b_up, (f, k)), ("dc", dc, (m, f)), ("gate", gate, (m, f)),
-              ("up", up, (m, f))]
-    wanted += [(name, t, shape) for name, t, shape in (("da", da, (m, k)), ("db_gate", db_gate, (f, k)),
-                                                       ("db_up", db_up, (f, k))) if t is not None]
-    if len(wanted) == 5:
+    m, k = _check_first("a", a, _HALF_TYPES)
+    dtype, device, f = a.dtype, a.device, _rows(b_gate)
+    if da is None and db_gate is None and db_up is None:
         raise ValueError("at least one of da, db_gate and db_up must be given")
-    for name, t, shape in wanted:
-        _check_matrix(name, t, shape, a.dtype, a.device)
-    nbytes = _load().beam_gated_gemmrc_backward_workspace_bytes(m, f, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
-    _call("beam_gated_gemmrc_backward", a.device, dc.data_ptr(), a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(),
+    _check_matrix("b_gate", b_gate, (f, k), dtype, device)
+    _check_matrix("b_up", b_up, (f, k), dtype, device)
+    _check_matrix("dc", dc, (m, f), dtype, device)
+    _check_matrix("gate", gate, (m, f), dtype, device)
+    _check_matrix("up", up, (m, f), dtype, device)
+    if da is not None:
+        _check_matrix("da", da, (m, k), dtype, device)
+    if db_gate is not None:
+        _check_matrix("db_gate", db_gate, (f, k), dtype, device)
+    if db_up is not None:
+        _check_matrix("db_up", db_up, (f, k), dtype, device)
+    nbytes = (_lib or _load()).beam_gated_gemmrc_backward_workspace_bytes(m, f, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _call("beam_gated_gemmrc_backward", device, dc.data_ptr(), a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(),
           gate.data_ptr(), up.data_ptr(), _ptr(da), _ptr(db_gate), _ptr(db_up), m, f, k, act, _half_flags(a),
           ws.data_ptr(), nbytes)
 
@@ -469,19 +493,17 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
 def gemmrc_backward(dc, a, b, da=None, db=None):
     """Gradients of c = a @ b.T: da[M,K] = dc[M,N] @ b[N,K] and db[N,K] = dc.T @ a[M,K], in one launch.  All tensors
     float16 or all bfloat16; the gradients wanted are given (at least one) and overwritten; N and K multiples of 8."""
-    _check_matrix("a", a, None, _HALF_TYPES, None)
-    m, k = a.shape
-    _check_matrix("b", b, None, a.dtype, a.device)
-    n = b.shape[0]
-    _check_matrix("b", b, (n, k), a.dtype, a.device)
-    _check_matrix("dc", dc, (m, n), a.dtype, a.device)
+    m, k = _check_first("a", a, _HALF_TYPES)
+    dtype, device, n = a.dtype, a.device, _rows(b)
+    _check_matrix("b", b, (n, k), dtype, device)
+    _check_matrix("dc", dc, (m, n), dtype, device)
     if da is None and db is None:
         raise ValueError("at least one of da and db must be given")
     if da is not None:
-        _check_matrix("da", da, (m, k), a.dtype, a.device)
+        _check_matrix("da", da, (m, k), dtype, device)
     if db is not None:
-        _check_matrix("db", db, (n, k), a.dtype, a.device)
-    _call("beam_gemmrc_backward", a.device, dc.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(da), _ptr(db), m, n, k,
+        _check_matrix("db", db, (n, k), dtype, device)
+    _call("beam_gemmrc_backward", device, dc.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(da), _ptr(db), m, n, k,
           _half_flags(a))
 
 
@@ -512,14 +534,17 @@ def mxfp4_tile_scales(scales):
     return whole.view(rb, 4, 32, cb, 4).permute(0, 3, 2, 1, 4).reshape(rb, cb, 512).contiguous()
 
 
-def _check_mxfp4(name, q, scales, device=None):
-    """(rows, k) of a quantised matrix."""
-    _check_matrix(name, q, None, torch.uint8, device)
-    rows, k = q.shape[0], q.shape[1] * 2
+_BYTES = (torch.uint8,)
+
+
+def _check_mxfp4(name, q, scales):
+    """(rows, k, device) of a quantised matrix."""
+    rows, half = _check_first(name, q, _BYTES)
+    k, device = 2 * half, q.device
     if k % 32:
         raise ValueError("%s must hold a multiple of 32 elements per row, got %d" % (name, k))
-    _check_matrix(name + "'s scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, q.device)
-    return rows, k
+    _check_matrix(name + "'s scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, device)
+    return rows, k, device
 
 
 def mxfp4_quantize(x, q, scales):
@@ -527,30 +552,37 @@ def mxfp4_quantize(x, q, scales):
 
     The scale of 32 elements is 2 to the power floor(log2(max |x|)) - 2; elements are rounded to the nearest of 0, 0.5, 1, 1.5,
     2, 3, 4, 6 times it, ties to even codes, and magnitudes above 6 become 6.  A block with an infinity or a NaN becomes NaN."""
-    _check_matrix("x", x, None, _HALF_TYPES, None)
-    rows, k = _check_mxfp4("q", q, scales, x.device)
-    _check_matrix("x", x, (rows, k), _HALF_TYPES, None)
-    _call("beam_mxfp4_quantize", x.device, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, k, _half_flags(x))
+    rows, k = _check_first("x", x, _HALF_TYPES)
+    device = x.device
+    if k % 32:
+        raise ValueError("x must hold a multiple of 32 elements per row, got %d" % k)
+    _check_matrix("q", q, (rows, k // 2), torch.uint8, device)
+    _check_matrix("scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, device)
+    _call("beam_mxfp4_quantize", device, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, k, _half_flags(x))
+
+
+_MXFP4_OUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
 def mxfp4_dequantize(q, scales, x):
     """The values of an MXFP4 matrix in x [rows, k], float16, bfloat16 or float32 (exact in the latter two)."""
-    rows, k = _check_mxfp4("q", q, scales)
-    _check_matrix("x", x, (rows, k), _HALF_TYPES + (torch.float32,), q.device)
-    kind = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}[x.dtype]
-    _call("beam_mxfp4_dequantize", q.device, q.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, k, kind)
+    rows, k, device = _check_mxfp4("q", q, scales)
+    kind = _MXFP4_OUT.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    _check_matrix("x", x, (rows, k), tuple(_MXFP4_OUT) if kind is None else x.dtype, device)
+    _call("beam_mxfp4_dequantize", device, q.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, k, kind)
 
 
 def mxfp4_gemmrc(a, a_scales, b, b_scales, c):
     """c[M,N] = a @ b.T of two MXFP4 matrices a [M,K] and b [N,K] on the 4-bit tensor cores: fp32 accumulation, c (float16 or
     bfloat16) rounded once.  N a multiple of 8, K of 32.  Scale bytes outside the matrices must be 0, as mxfp4_quantize
     and mxfp4_tile_scales leave them."""
-    m, k = _check_mxfp4("a", a, a_scales)
-    n, kb = _check_mxfp4("b", b, b_scales, a.device)
-    if k != kb:
-        raise ValueError("a holds %d elements per row but b %d" % (k, kb))
-    _check_matrix("c", c, (m, n), _HALF_TYPES, a.device)
-    _call("beam_mxfp4_gemmrc", a.device, a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(),
+    m, k, device = _check_mxfp4("a", a, a_scales)
+    n = _rows(b)
+    _check_matrix("b", b, (n, k // 2), torch.uint8, device)
+    _check_matrix("b's scales", b_scales, _mxfp4_scales_shape(n, k), torch.uint8, device)
+    known = isinstance(c, torch.Tensor) and c.dtype in _HALF_TYPES
+    _check_matrix("c", c, (m, n), c.dtype if known else _HALF_TYPES, device)
+    _call("beam_mxfp4_gemmrc", device, a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(),
           c.data_ptr(), m, n, k, _half_flags(c))
 
 
