@@ -11,7 +11,7 @@ namespace {
 int check_matrix(int rows, int k) {
   if (rows <= 0 || k <= 0) return BEAM_ERR_INVALID_ARG;
   if (k % 32 != 0) return BEAM_ERR_ALIGNMENT;
-  // units of 128 elements are counted in 32 bits
+  // units of 128 elements, with their padding, are counted in 32 bits
   if (static_cast<long long>(ceil_div(rows, 128)) * 128 * ceil_div(k, 128) > (1ll << 31) - 1024)
     return BEAM_ERR_UNSUPPORTED;
   return BEAM_OK;
@@ -19,15 +19,14 @@ int check_matrix(int rows, int k) {
 
 size_t packed_bytes(int rows, int k) { return static_cast<size_t>(rows) * (k / 2); }
 
-struct Units {
-  uint32_t kblocks, units;
-  int grid;
-};
-Units count_units(int rows, int k) {
-  Units u;
+// Lays a grid of 256-thread blocks, 64 units of 128 elements each, over rows x K: as many blocks of K side by side as fit.
+MxUnits lay_units(int rows, int k, int* grid) {
+  MxUnits u = {};
+  u.rows = rows;
   u.kblocks = static_cast<uint32_t>(ceil_div(k, 128));
-  u.units = static_cast<uint32_t>(rows) * u.kblocks;
-  u.grid = static_cast<int>((u.units + 16 * kMxUnits - 1) / (16 * kMxUnits));
+  while (u.kb_shift < 4 && (1u << u.kb_shift) < u.kblocks) ++u.kb_shift;
+  u.x_blocks = (u.kblocks + (1u << u.kb_shift) - 1) >> u.kb_shift;
+  *grid = static_cast<int>(u.x_blocks) * ceil_div(rows, kMxUnits * 16 >> u.kb_shift);
   return u;
 }
 
@@ -89,17 +88,15 @@ int launch_mxfp4_quantize(const void* x, void* q, void* scales, int rows, int k,
   if (overlap(x, xb, q, qb) || overlap(x, xb, scales, sb) || overlap(q, qb, scales, sb)) return BEAM_ERR_INVALID_ARG;
   DeviceCtx* ctx = current_device_ctx(&st);
   if (!ctx) return st;
-  const Units u = count_units(ceil_div(rows, 128) * 128, k);
   MxQuantParams p = {};
+  int grid = 0;
   p.x = static_cast<const uint4*>(x);
   p.q = static_cast<uint32_t*>(q);
-  p.scales = static_cast<uint32_t*>(scales);
+  p.scales = static_cast<uint8_t*>(scales);
   p.rows = rows;
   p.k = k;
-  p.kblocks = u.kblocks;
-  p.units = u.units;
-  p.bf16 = bf16;
-  return launch_dependent(bf16 ? mxfp4_quantize_kernel<true> : mxfp4_quantize_kernel<false>, u.grid, 256, 0, 1, stream,
+  p.units = lay_units(ceil_div(rows, 128) * 128, k, &grid);
+  return launch_dependent(bf16 ? mxfp4_quantize_kernel<true> : mxfp4_quantize_kernel<false>, grid, 256, 0, 1, stream,
                           "cudaLaunchKernelEx(mxfp4_quantize)", p);
 }
 
@@ -113,13 +110,14 @@ int launch_mxfp4_dequantize(const void* q, const void* scales, void* x, int rows
     return BEAM_ERR_INVALID_ARG;
   DeviceCtx* ctx = current_device_ctx(&st);
   if (!ctx) return st;
-  const Units u = count_units(rows, k);
+  int grid = 0;
+  const MxUnits u = lay_units(rows, k, &grid);
   auto kernel = type == kMxFp32   ? mxfp4_dequantize_kernel<kMxFp32>
                 : type == kMxBf16 ? mxfp4_dequantize_kernel<kMxBf16>
                                   : mxfp4_dequantize_kernel<kMxFp16>;
-  return launch_dependent(kernel, u.grid, 256, 0, 1, stream, "cudaLaunchKernelEx(mxfp4_dequantize)",
-                          static_cast<const uint32_t*>(q), static_cast<const uint32_t*>(scales), static_cast<uint4*>(x),
-                          rows, k, u.kblocks, u.units);
+  return launch_dependent(kernel, grid, 256, 0, 1, stream, "cudaLaunchKernelEx(mxfp4_dequantize)",
+                          static_cast<const uint32_t*>(q), static_cast<const uint8_t*>(scales), static_cast<uint4*>(x), k,
+                          u);
 }
 
 int launch_mxfp4_gemmrc(const void* A, const void* a_scales, const void* B, const void* b_scales, void* C, int m, int n,

@@ -16,74 +16,89 @@ namespace beam {
 // One half-warp takes 128 elements of a row (a row of one scale block): each lane 8 elements, four lanes a scale.
 //   s = floor(log2(max |x|)) - 2, at least -127: the exponent field of the largest magnitude, without a logarithm;
 //   q = x 2^-s rounded to the nearest e2m1 value, ties to even; magnitudes above 6 (up to 8 by the choice of s) become 6.
-// The scaling is exact in fp32.  A block with an infinity or a NaN gets the NaN scale.  Bound by memory: 2 bytes in and
-// 17/32 out per element; each thread keeps kUnits 16-byte loads in flight.
-struct MxQuantParams {
-  const uint4* x;
-  uint32_t* q;       // 8 codes per word
-  uint32_t* scales;  // 4 scales per word
-  int rows, k;
-  uint32_t kblocks;  // ceil(k / 128)
-  uint32_t units;    // rows padded to 128, times kblocks
-  int bf16;
+// The scaling is exact in fp32.  A block with an infinity or a NaN gets the NaN scale.  Bound by memory (2 bytes in and
+// 17/32 out per element) as long as the instructions per element stay few: magnitudes are compared as pairs of 16-bit integers
+// (infinities and NaN order above all finite values), and a block's half-warps are laid over rows and K by shifts.
+// A block of 256 threads covers 2^kb_shift blocks of K x (64 >> kb_shift) rows: its 16 half-warps lie side by side over K and then
+// over rows, and each takes kMxUnits rows at equal distances, so a thread's addresses differ by constants.
+struct MxUnits {
+  int rows;           // rows that units are laid over (quantisation: rounded up to 128, the padding of the scales is written too)
+  uint32_t kblocks;   // ceil(k / 128)
+  uint32_t kb_shift;  // at most 4
+  uint32_t x_blocks;  // ceil(kblocks / 2^kb_shift)
 };
 
-constexpr int kMxUnits = 4;
+constexpr int kMxUnits = 4;  // units per half-warp: 16-byte loads in flight per thread
 
-__device__ __forceinline__ size_t mx_scale_word(uint32_t row, uint32_t kb, uint32_t kblocks) {
-  return (static_cast<size_t>(row >> 7) * kblocks + kb) * 128 + (row & 31) * 4 + ((row >> 5) & 3);
+struct MxPlace {
+  uint32_t row, step;   // unit i works on row + i step
+  uint32_t kb, col;     // its block of K and this lane's first column
+};
+__device__ __forceinline__ MxPlace mx_place(const MxUnits& u) {
+  const uint32_t half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const uint32_t by = blockIdx.x / u.x_blocks, bx = blockIdx.x - by * u.x_blocks;
+  MxPlace p;
+  p.kb = (bx << u.kb_shift) + (half & ((1u << u.kb_shift) - 1u));
+  p.step = 16u >> u.kb_shift;
+  p.row = by * (kMxUnits * p.step) + (half >> u.kb_shift);
+  p.col = p.kb * 128 + lane * 8;
+  return p;
 }
+// First byte of a block's scales, and the word of a row in it.  A thread's rows lie in one group of 128.
+__device__ __forceinline__ size_t mx_scale_block(const MxPlace& p, uint32_t kblocks) {
+  return (static_cast<size_t>(p.row >> 7) * kblocks + p.kb) * 512;
+}
+__device__ __forceinline__ uint32_t mx_scale_row(uint32_t row) { return (row & 31) * 16 + ((row >> 5) & 3) * 4; }
+
+struct MxQuantParams {
+  const uint4* x;
+  uint32_t* q;      // 8 codes per word
+  uint8_t* scales;
+  int rows, k;
+  MxUnits units;
+};
 
 template <bool kBf16>
 static __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxQuantParams p) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  const uint32_t lane = threadIdx.x & 15;
-  const uint32_t first = blockIdx.x * (16 * kMxUnits) + (threadIdx.x >> 4);
+  const MxPlace at = mx_place(p.units);
+  const bool in_k = at.col < static_cast<uint32_t>(p.k);
+  const size_t first = (static_cast<size_t>(at.row) * p.k + at.col) >> 3, step = (static_cast<size_t>(at.step) * p.k) >> 3;
+  const uint4* from = p.x + first;
   uint4 x[kMxUnits];
-  uint32_t row[kMxUnits], kb[kMxUnits];
-  bool live[kMxUnits];
 #pragma unroll
   for (int i = 0; i < kMxUnits; ++i) {
-    const uint32_t u = first + 16 * i;
-    row[i] = u / p.kblocks;
-    kb[i] = u - row[i] * p.kblocks;
-    const uint32_t col = kb[i] * 128 + lane * 8;
-    live[i] = u < p.units && row[i] < static_cast<uint32_t>(p.rows) && col < static_cast<uint32_t>(p.k);
     x[i] = make_uint4(0, 0, 0, 0);
-    if (live[i]) x[i] = __ldcs(p.x + (static_cast<size_t>(row[i]) * p.k + col) / 8);
+    if (in_k && at.row + i * at.step < static_cast<uint32_t>(p.rows)) x[i] = __ldcs(from + i * step);
   }
+  uint32_t* to = p.q + first;
+  uint8_t* scales = p.scales + mx_scale_block(at, p.units.kblocks) + ((threadIdx.x & 15) >> 2);
+  const bool writes_scale = (threadIdx.x & 3) == 0 && at.kb < p.units.kblocks;
 #pragma unroll
   for (int i = 0; i < kMxUnits; ++i) {
+    const uint32_t row = at.row + i * at.step;
     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = max(top & 0xFFFFu, top >> 16);
+    // the exponent field that the largest magnitude has in fp32; 255 for infinities and NaN, whose codes do not matter
+    const uint32_t field = kBf16 ? top >> 7 : __float_as_uint(ptx::unpack_in2(top, 0).x) >> 23;
+    uint32_t scale = max(field, 2u) - 2u;
+    const float inv = __uint_as_float((254u - scale) << 23);  // 2^-s
+    if (field == 255) scale = 255;
     float v[8];
-    uint32_t top = 0;  // magnitudes compare as integers; infinities and NaN above all finite values
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = ptx::unpack_in2(w[j], kBf16);
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-      top = max(top, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
+      v[2 * j] = f.x * inv;
+      v[2 * j + 1] = f.y * inv;
     }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t field = top >> 23;
-    uint32_t scale = field > 2 ? field - 2 : 0;
-    // 2^-s: exponent field 254 - scale, between 2 and 254
-    float inv = __uint_as_float((254u - scale) << 23);
-    if (field == 255) {
-      scale = 255;
-      inv = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = field == 255 ? 0.f : v[j] * inv;
     const uint32_t code = ptx::pack_e2m1x8(v);
-    if (live[i]) p.q[(static_cast<size_t>(row[i]) * p.k + kb[i] * 128 + lane * 8) / 8] = code;
-    // the half-warp's four scales as one word; lanes past K hold zeros and so give scale 0
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) word |= __shfl_sync(0xffffffffu, scale, j * 4, 16) << (8 * j);
-    if (lane == 0 && first + 16 * i < p.units) p.scales[mx_scale_word(row[i], kb[i], p.kblocks)] = word;
+    if (in_k && row < static_cast<uint32_t>(p.rows)) to[i * step] = code;
+    // lanes past K hold zeros and so give the scale 0
+    if (writes_scale && row < static_cast<uint32_t>(p.units.rows)) scales[mx_scale_row(row)] = static_cast<uint8_t>(scale);
   }
 }
 
@@ -92,42 +107,41 @@ enum MxType : int { kMxFp16 = 0, kMxBf16 = 1, kMxFp32 = 2 };
 // The inverse: x = q 2^s, exact in fp32 and rounded to the output type.  Same units.
 template <int kType>
 static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* __restrict__ q,
-                                                                      const uint32_t* __restrict__ scales,
-                                                                      uint4* __restrict__ x, int rows, int k,
-                                                                      uint32_t kblocks, uint32_t units) {
+                                                                      const uint8_t* __restrict__ scales,
+                                                                      uint4* __restrict__ x, int k, MxUnits units) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  const uint32_t lane = threadIdx.x & 15;
-  const uint32_t first = blockIdx.x * (16 * kMxUnits) + (threadIdx.x >> 4);
-  uint32_t code[kMxUnits], word[kMxUnits];
-  size_t at[kMxUnits];
-  bool live[kMxUnits];
+  const MxPlace at = mx_place(units);
+  if (at.col >= static_cast<uint32_t>(k)) return;
+  const size_t first = (static_cast<size_t>(at.row) * k + at.col) >> 3, step = (static_cast<size_t>(at.step) * k) >> 3;
+  scales += mx_scale_block(at, units.kblocks) + ((threadIdx.x & 15) >> 2);
+  uint32_t code[kMxUnits], byte[kMxUnits];
 #pragma unroll
   for (int i = 0; i < kMxUnits; ++i) {
-    const uint32_t u = first + 16 * i;
-    const uint32_t row = u / kblocks, kb = u - row * kblocks, col = kb * 128 + lane * 8;
-    live[i] = u < units && col < static_cast<uint32_t>(k);
-    at[i] = (static_cast<size_t>(row) * k + col) / 8;
-    code[i] = live[i] ? __ldcs(q + at[i]) : 0u;
-    word[i] = live[i] ? __ldg(scales + mx_scale_word(row, kb, kblocks)) : 0u;
+    const uint32_t row = at.row + i * at.step;
+    code[i] = byte[i] = 0;
+    if (row < static_cast<uint32_t>(units.rows)) {
+      code[i] = __ldcs(q + first + i * step);
+      byte[i] = __ldg(scales + mx_scale_row(row));
+    }
   }
 #pragma unroll
   for (int i = 0; i < kMxUnits; ++i) {
-    if (!live[i]) continue;
-    const uint32_t s = (word[i] >> (8 * (lane >> 2))) & 255u;
+    if (at.row + i * at.step >= static_cast<uint32_t>(units.rows)) break;
     // 2^(s - 127) in fp32: 0 is the subnormal 2^-127, 255 a NaN
+    const uint32_t s = byte[i];
     const float scale = __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7FC00000u : s << 23);
     float v[8];
     ptx::unpack_e2m1x8(code[i], v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= scale;
     if constexpr (kType == kMxFp32) {
-      float4* dst = reinterpret_cast<float4*>(x) + 2 * at[i];
+      float4* dst = reinterpret_cast<float4*>(x) + 2 * (first + i * step);
       __stcs(dst, make_float4(v[0], v[1], v[2], v[3]));
       __stcs(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
     } else {
-      __stcs(x + at[i], make_uint4(ptx::pack_out2(v[0], v[1], kType), ptx::pack_out2(v[2], v[3], kType),
-                                   ptx::pack_out2(v[4], v[5], kType), ptx::pack_out2(v[6], v[7], kType)));
+      __stcs(x + first + i * step, make_uint4(ptx::pack_out2(v[0], v[1], kType), ptx::pack_out2(v[2], v[3], kType),
+                                              ptx::pack_out2(v[4], v[5], kType), ptx::pack_out2(v[6], v[7], kType)));
     }
   }
 }
