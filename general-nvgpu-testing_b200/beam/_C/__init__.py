@@ -519,7 +519,7 @@ def mxfp4_empty(rows, k, device=None):
         raise ValueError("rows must be positive and k a positive multiple of 32, got %d, %d" % (rows, k))
     device = torch.device("cuda") if device is None else device
     return (torch.empty(rows, k // 2, dtype=torch.uint8, device=device),
-            torch.empty(_mxfp4_scales_shape(rows, k), dtype=torch.uint8, device=device))
+            torch.empty(*_mxfp4_scales_shape(rows, k), dtype=torch.uint8, device=device))
 
 
 def mxfp4_tile_scales(scales):

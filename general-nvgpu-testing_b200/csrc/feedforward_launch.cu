@@ -64,6 +64,8 @@ int launch_gated_instance(DeviceCtx* ctx, const GatedPlan& plan, int resident, c
   p.stage_bytes = S::kABytes + p.width * 128 * (kCta == 2 ? 1 : 2);
   p.stages = S::kRingBytes / p.stage_bytes;
   if (p.stages > S::kMaxStages) p.stages = S::kMaxStages;
+  p.issuers = p.width <= 64 && k > S::kBK ? 2 : 1;  // UMMAs of N <= 128; every tile gives each of the two a k-block
+  if (p.issuers == 2) p.stages &= ~1;
   p.m_tiles = ceil_div(m, S::kBM * kCta);
   p.n_tiles = ceil_div(f, p.width);
   p.group_m = 8;

@@ -17,7 +17,7 @@
 //              stages; only the rows of A that exist are loaded (the other lanes of the UMMA compute on leftovers that
 //              are never stored); C is small and written straight from registers.
 //
-// Roles: warp 0 TMA producer, warp 1 MMA issuer, warps 2..5 epilogue.
+// Roles: warp 0 and warps 6 on TMA producers, warp 1 and the last warp MMA issuers, warps 2..5 epilogue.
 #pragma once
 
 #include "activation.cuh"
@@ -36,6 +36,7 @@ struct GatedParams {
   int a_rows;             // rows of A that a CTA loads
   int stages, stage_bytes;
   int m_tiles, n_tiles, group_m;
+  int issuers;            // warps that issue UMMAs: 1, or 2 with an accumulator each, taking turns at the k-blocks
   int act;
   int bf16;
   int* status;
@@ -48,8 +49,10 @@ struct GatedShape {
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kMaxStages = 8;
   static constexpr int kProducers = kCta == 1 ? 4 : 2;
-  static constexpr int kThreads = 32 * (5 + kProducers);
-  static constexpr int kAccCols = 256;  // TMEM columns between the two accumulators
+  static constexpr int kSecondIssuer = 5 + kProducers;  // its warp
+  static constexpr int kThreads = 32 * (6 + kProducers);
+  static constexpr int kAccCols = 256;    // TMEM columns from one tile's accumulator to the next tile's
+  static constexpr int kChainCols = 128;  // from the first issuer's to the second's
   static constexpr int kBufsPerWarp = 4;
   static constexpr int kStoreBufBytes = 32 * 64;
   static constexpr int kStagingBytes = kCta == 2 ? 4 * kBufsPerWarp * kStoreBufBytes : 0;
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
       ptx::mbar_init(empty_bar(s), 1);
     }
     for (uint32_t a = 0; a < 2; ++a) {
-      ptx::mbar_init(tmem_full_bar(a), 1);
+      ptx::mbar_init(tmem_full_bar(a), static_cast<uint32_t>(p.issuers));
       ptx::mbar_init(tmem_empty_bar(a), 4 * kCta);  // one arrive per epilogue warp of each CTA
     }
     *cta_abort = 0;
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0 || warp >= 6) {
+  if (warp == 0 || (warp >= 6 && warp < S::kSecondIssuer)) {
     // ------------------------------------------------------------------ TMA producers
     ptx::grid_dependency_wait();  // before the first global read; everything else follows from these reads
     const uint32_t b_bytes = static_cast<uint32_t>(p.width) * 128u;
@@ -179,44 +182,52 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
       if (kb < num_kb) break;  // a wait ran out
       kb -= num_kb;
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (leader) {
+  } else if (warp == 1 || warp == S::kSecondIssuer) {
+    // ------------------------------------------------------------------ MMA issuers
+    // One warp needs about 380 cycles for a k-block's four UMMAs, their commit and its waits, more than the tensor pipe does
+    // when N <= 128.  For those tiles two warps take turns at the k-blocks, each into an accumulator of its own (the
+    // epilogue adds the two, always in the same order).  Which warp has a k-block goes by its number in the CTA's whole walk
+    // and the ring is an even number of stages deep, so a stage always belongs to the same warp: a parity wait cannot mistake
+    // one use of a stage for the one two uses earlier.
+    const uint32_t issuers = static_cast<uint32_t>(p.issuers);
+    const uint32_t mine = warp == 1 ? 0u : 1u;
+    if (leader && mine < issuers) {
       const uint32_t idesc =
           ptx::umma_idesc_f16_f32(S::kBM * kCta, 2 * p.width) | (p.bf16 ? ptx::kIdescBf16Inputs : 0u);
       const uint64_t a_desc0 = ptx::umma_desc_k_sw128(smem_base);
       const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + S::kABytes);
       const uint64_t desc_stride = static_cast<uint64_t>(p.stage_bytes >> 4);
       const uint32_t stages = static_cast<uint32_t>(p.stages);
-      uint32_t s = 0, ph = 0;
-      bool alive = true;
-      for (int t = first, j = 0; alive && t < tiles; t += stride, ++j) {
+      uint32_t s = mine, ph = 0;
+      int kb = static_cast<int>(mine);
+      for (int t = first, j = 0; t < tiles; t += stride, ++j) {
         const uint32_t acc = static_cast<uint32_t>(j) & 1u;
         const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
         if (!bounded_wait_converged(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc, lane)) break;
         ptx::tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * S::kAccCols;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) {
-            alive = false;
-            break;
-          }
+        const uint32_t d_tmem = tmem_base + acc * S::kAccCols + mine * S::kChainCols;
+        const int kb_first = kb;
+        for (; kb < num_kb; kb += static_cast<int>(issuers)) {
+          if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) break;
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
             ptx::umma_f16_kblock<kCta>(d_tmem, a_desc0 + s * desc_stride, b_desc0 + s * desc_stride, idesc,
-                                       kb > 0 ? 1u : 0u);
+                                       kb > kb_first ? 1u : 0u);
             if constexpr (kCta == 1)
               ptx::umma_commit<1>(empty_bar(s));
             else
               ptx::umma_commit_pair_both(empty_bar(s), 0x3);
           }
           __syncwarp();
-          if (++s == stages) {
-            s = 0;
+          s += issuers;
+          if (s >= stages) {
+            s -= stages;
             ph ^= 1u;
           }
         }
-        if (alive && ptx::elect_one()) {
+        if (kb < num_kb) break;  // a wait ran out
+        kb -= num_kb;
+        if (ptx::elect_one()) {
           if constexpr (kCta == 1)
             ptx::umma_commit<1>(tmem_full_bar(acc));
           else
@@ -247,6 +258,17 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
         ptx::tmem_ld_32x32(taddr + c, g);  // a narrow tile's last read runs into the neighbouring columns: not stored
         ptx::tmem_ld_32x32(taddr + p.width + c, u);
         ptx::tmem_ld_wait();
+        if (p.issuers == 2) {  // the second issuer's sums
+          uint32_t x[32];
+          ptx::tmem_ld_32x32(taddr + S::kChainCols + c, x);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 32; ++q) g[q] = __float_as_uint(__uint_as_float(g[q]) + __uint_as_float(x[q]));
+          ptx::tmem_ld_32x32(taddr + S::kChainCols + p.width + c, x);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(__uint_as_float(u[q]) + __uint_as_float(x[q]));
+        }
         // Writes 32 columns of output `which`, rounded once.
         auto store = [&](const uint32_t(&v)[32], int which) {
           uint32_t o[16];

@@ -67,7 +67,7 @@ int launch_instance(DeviceCtx* ctx, const void* A, const void* sa, const void* B
   if (st != BEAM_OK) return st;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
   const int clusters = tiles < resident ? static_cast<int>(tiles) : resident;
-  const int smem = p.stages * p.stage_bytes + S::kStagingBytes + S::kBarBytes + 1024;
+  const int smem = p.stages * p.stage_bytes + S::kStagingBytes + S::kBarBytes;
   return launch_dependent(mxfp4_umma_kernel<kCta>, clusters * kCta, S::kThreads, smem, kCta, stream,
                           "cudaLaunchKernelEx(mxfp4_umma)", p);
 }

@@ -188,10 +188,11 @@ struct MxShape {
   static constexpr int kMaxWidth = kCta == 2 ? 256 : 128;
   static constexpr int kAccStep = kCta == 2 ? 192 : 128;  // TMEM columns from one accumulator to the other
   static constexpr int kScaleCols = kAccStep + kMaxWidth;  // first column of the scales: two sets of 2 x (4 + 8)
-  static constexpr int kStagingBytes = kCta == 2 ? 4 * 2 * 4096 : 0;
+  static constexpr int kBufsPerWarp = 1;
+  static constexpr int kStagingBytes = kCta == 2 ? 4 * kBufsPerWarp * 4096 : 0;
   static constexpr int kBarBytes = 256;
   static constexpr int kSmemLimit = 232448;
-  static constexpr int kRingBytes = kSmemLimit - 1024 - kStagingBytes - kBarBytes;
+  static constexpr int kRingBytes = kSmemLimit - kStagingBytes - kBarBytes;
   static_assert(kScaleCols + 2 * 24 <= 512, "accumulators and scales share 512 columns");
   static_assert((2 * kMaxStages + 4) * 8 + 8 <= kBarBytes, "barrier block too small");
 };
@@ -199,7 +200,7 @@ struct MxShape {
 template <int kCta>
 __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(const __grid_constant__ MxGemmParams p) {
   using S = MxShape<kCta>;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_tiles[];
   const uint32_t warp = ptx::warp_index();
   const uint32_t lane = threadIdx.x & 31;
   const int cta_rank = (kCta == 2) ? static_cast<int>(ptx::cluster_ctarank()) : 0;
@@ -209,8 +210,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
   const int tiles = p.m_tiles * p.n_tiles;
   const int num_kb = (p.k + S::kBK - 1) / S::kBK;
 
-  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const uint32_t smem_base = ptx::smem_u32(smem_tiles);
   const uint32_t ring_bytes = static_cast<uint32_t>(p.stages * p.stage_bytes);
   const uint32_t b_bytes = static_cast<uint32_t>(p.width / kCta) * 128u;
   const uint32_t staging_base = smem_base + ring_bytes;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
   auto tmem_full_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + a); };
   auto tmem_empty_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + 2 + a); };
   volatile uint32_t* tmem_slot =
-      reinterpret_cast<volatile uint32_t*>(smem_gen + ring_bytes + S::kStagingBytes + 8 * (2 * S::kMaxStages + 4));
+      reinterpret_cast<volatile uint32_t*>(smem_tiles + ring_bytes + S::kStagingBytes + 8 * (2 * S::kMaxStages + 4));
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   auto tile_at = [&](int t, int& mt, int& nt) {
@@ -423,9 +423,9 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
             out[q] = ptx::pack_out2(__uint_as_float(v0[2 * q]), __uint_as_float(v0[2 * q + 1]), p.bf16);
             out[16 + q] = ptx::pack_out2(__uint_as_float(v1[2 * q]), __uint_as_float(v1[2 * q + 1]), p.bf16);
           }
-          const uint32_t buf = staging_base + (quad * 2u + (stores & 1u)) * 4096u;
-          if (stores >= 2) {
-            if (lane == 0) ptx::tma_store_wait_read<1>();
+          const uint32_t buf = staging_base + (quad * S::kBufsPerWarp + stores % S::kBufsPerWarp) * 4096u;
+          if (stores >= S::kBufsPerWarp) {
+            if (lane == 0) ptx::tma_store_wait_read<S::kBufsPerWarp - 1>();
             __syncwarp();
           }
 #pragma unroll
