@@ -10,26 +10,40 @@ namespace beam {
 namespace {
 
 struct GatedPlan {
-  int ctas;   // per tile
-  int width;  // columns of F per tile
+  int ctas;       // per tile
+  int width;      // columns of F per tile
+  int split = 1;  // CTAs that share a tile's contraction (single-CTA tiles only)
 };
 
 // Up to 128 rows one CTA's tile holds them all and the weights are read once whatever the width, so the width only deals out F:
-// the smallest multiple of 8 with which the columns take as few waves of all SMs as 128-wide tiles would.
+// the smallest multiple of 8 with which the columns take as few waves of all SMs as 128-wide tiles would.  While that
+// leaves a CTA more k-blocks than bytes (a k-block takes its issuers about 0.14 us, in which an SM can read a width of 28),
+// clusters of 2 or 4 CTAs share a tile's contraction: wider tiles over fewer k-blocks, for an exchange of sums at the end.  Measured,
+// one row, us with 1 / 2 / 4 CTAs: F = 512, K = 4096 11.2 / 9.0 / 8.5; 2048, 4096 12.0 / 10.9 / 12.1; 4096, 4096 14.9 / 15.7 / 17.2;
+// 1024, 8192 18.6 / 13.3 / 12.2; 1024, 2048 7.7 / 7.3 / 7.7; 512, 1024 6.0 / 6.4 / 7.2.
 //
 // Above, pairs work on 256 rows.  A wave of narrower tiles is shorter, but not in proportion (A is read as often, and a UMMA
 // of N <= 128 is bound by its issue); measured per wave at K = 4096, in percent of a wave of 128-wide tiles: 96 columns 73 alone
 // and 78 among many waves, 64 columns 60, 32 columns 55.  The width with the least total is taken, the wider of two
 // that are equal: 128 for all large problems (4096 x 16384 x 4096: 681 us against 697 with 96 and 823 with 64), the narrowest
 // that still takes one wave for small ones (256 x 2048 x 2048: 11.1 us with 32 against 16.2 with 128).
-GatedPlan gated_plan(int m, int f, int sm_count, int pairs) {
+GatedPlan gated_plan(int m, int f, int k, const int (&fit)[4]) {
   GatedPlan plan;
   if (m <= 128) {
     plan.ctas = 1;
-    const int waves = ceil_div(f, 128 * sm_count);
-    plan.width = (ceil_div(f, waves * sm_count) + 7) / 8 * 8;
+    const int waves = ceil_div(f, 128 * fit[0]);
+    plan.width = (ceil_div(f, waves * fit[0]) + 7) / 8 * 8;
+    const int num_kb = ceil_div(k, 64);
+    const int split = plan.width <= 8 && num_kb >= 48 ? 4 : plan.width <= 16 && num_kb >= 32 ? 2 : 1;
+    const int step = 8 * split;  // every CTA finishes a multiple of 8 columns
+    const int shared_width = (ceil_div(f, fit[split / 2]) + step - 1) / step * step;
+    if (split > 1 && shared_width <= 128) {
+      plan.split = split;
+      plan.width = shared_width;
+    }
     return plan;
   }
+  const int pairs = fit[3];
   plan.ctas = 2;
   const int widths[4] = {128, 96, 64, 32}, wave_cost[4] = {100, 80, 61, 55};
   long long best = 0;
@@ -61,13 +75,20 @@ int launch_gated_instance(DeviceCtx* ctx, const GatedPlan& plan, int resident, c
   p.out[2] = U;
   p.status = ctx->status_word;
   p.a_rows = kCta == 2 ? S::kBM : (m + 7) / 8 * 8;
-  p.stage_bytes = S::kABytes + p.width * 128 * (kCta == 2 ? 1 : 2);
-  p.stages = S::kRingBytes / p.stage_bytes;
-  if (p.stages > S::kMaxStages) p.stages = S::kMaxStages;
-  p.issuers = p.width <= 64 && k > S::kBK ? 2 : 1;  // UMMAs of N <= 128; every tile gives each of the two a k-block
-  if (p.issuers == 2) p.stages &= ~1;
+  p.a_bytes = p.a_rows * 128;
+  p.stage_bytes = p.a_bytes + p.width * 128 * (kCta == 2 ? 1 : 2);
   p.m_tiles = ceil_div(m, S::kBM * kCta);
   p.n_tiles = ceil_div(f, p.width);
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  const int clusters = tiles < resident ? static_cast<int>(tiles) : resident;
+  p.split = plan.split;
+  // Two issuers for UMMAs of N <= 128; every CTA must have a k-block for each.
+  p.issuers = p.width <= 64 && k > S::kBK * p.split * 2 ? 2 : 1;
+  // A UMMA reads 128 rows of A whether they were loaded or not: behind the last stage there is room for them.
+  const int a_slack = S::kABytes - p.a_bytes;
+  p.stages = (S::kRingBytes - a_slack) / p.stage_bytes;
+  if (p.stages > S::kMaxStages) p.stages = S::kMaxStages;
+  if (p.issuers == 2) p.stages &= ~1;
   p.group_m = 8;
   int st = encode_tmap_2d(&p.tm_a, A, 2, m, k, k, static_cast<uint32_t>(p.a_rows), S::kBK, true);
   if (st == BEAM_OK) st = encode_tmap_2d(&p.tm_gate, Bg, 2, f, k, k, static_cast<uint32_t>(p.width), S::kBK, true);
@@ -77,10 +98,12 @@ int launch_gated_instance(DeviceCtx* ctx, const GatedPlan& plan, int resident, c
       if (p.out[i]) st = encode_tmap_2d_sw64(&p.tm_out[i], p.out[i], m, f, f, 32, 32);
   }
   if (st != BEAM_OK) return st;
-  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-  const int clusters = tiles < resident ? static_cast<int>(tiles) : resident;
-  const int smem = p.stages * p.stage_bytes + S::kStagingBytes + S::kBarBytes + 1024;
-  return launch_dependent(gated_umma_kernel<kCta>, clusters * kCta, S::kThreads, smem, kCta, stream,
+  const int exchange = (p.split - 1) * (p.width / p.split) * 2 * 128 * 4;  // what the others of a cluster send
+  p.bar_offset = p.stages * p.stage_bytes + a_slack + S::kStagingBytes;
+  if (p.bar_offset < exchange) p.bar_offset = exchange;
+  const int smem = p.bar_offset + S::kBarBytes + 1024;
+  const int ctas = kCta * p.split;
+  return launch_dependent(gated_umma_kernel<kCta>, clusters * ctas, S::kThreads, smem, ctas, stream,
                           "cudaLaunchKernelEx(gated_umma)", p);
 }
 
@@ -111,17 +134,19 @@ int launch_gated(const void* A, const void* Bg, const void* Bu, void* C, void* G
   }
   DeviceCtx* ctx = current_device_ctx(&st);
   if (!ctx) return st;
-  static ResidentTable table[2];
-  int fit[2];
-  st = resident_grid(&table[0], gated_umma_kernel<1>, ctx, GatedShape<1>::kThreads, GatedShape<1>::kSmemLimit, 1, &fit[0]);
+  static ResidentTable table[4];
+  int fit[4];  // single CTAs; clusters of 2 and 4 CTAs that share a contraction; pairs
+  for (int i = 0; i < 3 && st == BEAM_OK; ++i)
+    st = resident_grid(&table[i], gated_umma_kernel<1>, ctx, GatedShape<1>::kThreads, GatedShape<1>::kSmemLimit, 1 << i,
+                       &fit[i]);
   if (st == BEAM_OK)
-    st = resident_grid(&table[1], gated_umma_kernel<2>, ctx, GatedShape<2>::kThreads, GatedShape<2>::kSmemLimit, 2,
-                       &fit[1]);
+    st = resident_grid(&table[3], gated_umma_kernel<2>, ctx, GatedShape<2>::kThreads, GatedShape<2>::kSmemLimit, 2,
+                       &fit[3]);
   if (st != BEAM_OK) return st;
-  const GatedPlan plan = gated_plan(m, f, fit[0], fit[1]);
-  return plan.ctas == 1
-             ? launch_gated_instance<1>(ctx, plan, fit[0], A, Bg, Bu, C, G, U, m, f, k, activation, bf16, stream)
-             : launch_gated_instance<2>(ctx, plan, fit[1], A, Bg, Bu, C, G, U, m, f, k, activation, bf16, stream);
+  const GatedPlan plan = gated_plan(m, f, k, fit);
+  return plan.ctas == 1 ? launch_gated_instance<1>(ctx, plan, plan.split == 1 ? fit[0] : plan.split == 2 ? fit[1] : fit[2], A,
+                                                   Bg, Bu, C, G, U, m, f, k, activation, bf16, stream)
+                        : launch_gated_instance<2>(ctx, plan, fit[3], A, Bg, Bu, C, G, U, m, f, k, activation, bf16, stream);
 }
 
 namespace {

@@ -12,12 +12,16 @@
 //
 // Two variants, chosen by rows (the rule and what it measured stand beside gated_plan() in feedforward_launch.cu):
 //   kCta = 2   M > 128: 256-row tiles, width 32, 64, 96 or 128, persistent grid, two TMEM accumulators, C stored by TMA.
+//              4096 x 16384 x 4096 (bf16): 657 us, 1674 TFLOP/s, as fast as a cuBLAS product of that size alone; bound by
+//              the tensor pipe and the power it draws.
 //   kCta = 1   M <= 128: the call is bound by reading the weights once.  The width is whatever multiple of 8 deals F
-//              to all SMs in one wave, so that every SM streams the same share of the weights through a ring of up to 8
-//              stages; only the rows of A that exist are loaded (the other lanes of the UMMA compute on leftovers that
-//              are never stored); C is small and written straight from registers.
+//              to all SMs in one wave, so that every SM streams the same share of the weights through a ring of up to 16
+//              stages; only the rows of A that exist are loaded and have room in a stage (the other lanes of the UMMA
+//              compute on what lies behind them, and are never stored); C is small and written straight from registers.
+//              One row, F = 16384, K = 4096: 45.4 us, 5.9 TB/s.  Halving the ring, so that the next launch's CTAs fit
+//              beside this one's, was slower for all shapes (8192 x 4096: 25.8 -> 27.8 us).
 //
-// Roles: warp 0 and warps 6 on TMA producers, warp 1 and the last warp MMA issuers, warps 2..5 epilogue.
+// Roles: warps 0 and 6 are TMA producers, warps 1 and 7 issue UMMAs, warps 2..5 are the epilogue.
 #pragma once
 
 #include "activation.cuh"
@@ -35,28 +39,32 @@ struct GatedParams {
   int width;              // columns of F per tile
   int a_rows;             // rows of A that a CTA loads
   int stages, stage_bytes;
+  int a_bytes;            // of a stage: B begins there
+  int bar_offset;         // the barriers' place in shared memory, behind the ring and what else takes its place
   int m_tiles, n_tiles, group_m;
   int issuers;            // warps that issue UMMAs: 1, or 2 with an accumulator each, taking turns at the k-blocks
+  int split;              // single CTAs: a cluster of this many CTAs shares each tile's contraction
   int act;
   int bf16;
   int* status;
 };
+
+constexpr int kGatedChainCols = 128;  // TMEM columns from the first issuer's accumulator to the second's
 
 template <int kCta>
 struct GatedShape {
   static constexpr int kBM = 128;
   static constexpr int kBK = 64;
   static constexpr int kABytes = kBM * kBK * 2;
-  static constexpr int kMaxStages = 8;
-  static constexpr int kProducers = kCta == 1 ? 4 : 2;
+  static constexpr int kMaxStages = 16;
+  static constexpr int kProducers = 2;  // at most the least depth of the ring
   static constexpr int kSecondIssuer = 5 + kProducers;  // its warp
   static constexpr int kThreads = 32 * (6 + kProducers);
   static constexpr int kAccCols = 256;    // TMEM columns from one tile's accumulator to the next tile's
-  static constexpr int kChainCols = 128;  // from the first issuer's to the second's
   static constexpr int kBufsPerWarp = 4;
   static constexpr int kStoreBufBytes = 32 * 64;
   static constexpr int kStagingBytes = kCta == 2 ? 4 * kBufsPerWarp * kStoreBufBytes : 0;
-  static constexpr int kBarBytes = 256;
+  static constexpr int kBarBytes = 512;
   static constexpr int kSmemLimit = 232448;
   static constexpr int kRingBytes = kSmemLimit - 1024 - kStagingBytes - kBarBytes;
   static_assert((2 * kMaxStages + 4) * 8 + 8 <= kBarBytes, "barrier block too small");
@@ -77,6 +85,35 @@ __device__ __forceinline__ void gated_combine(int act, uint32_t (&g)[32], const 
   }
 }
 
+// 32 columns of both products from TMEM, the two issuers' sums added where there are two.
+__device__ __forceinline__ void gated_load(const GatedParams& p, uint32_t taddr, uint32_t (&g)[32], uint32_t (&u)[32]) {
+  ptx::tmem_ld_32x32(taddr, g);
+  ptx::tmem_ld_32x32(taddr + p.width, u);
+  ptx::tmem_ld_wait();
+  if (p.issuers == 2) {
+    uint32_t x[32];
+    ptx::tmem_ld_32x32(taddr + kGatedChainCols, x);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int q = 0; q < 32; ++q) g[q] = __float_as_uint(__uint_as_float(g[q]) + __uint_as_float(x[q]));
+    ptx::tmem_ld_32x32(taddr + kGatedChainCols + p.width, x);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(__uint_as_float(u[q]) + __uint_as_float(x[q]));
+  }
+}
+
+// One row's share of up to 32 columns, packed, straight to output `which`; columns is a multiple of 8, as is F.
+__device__ __forceinline__ void gated_store_row(const GatedParams& p, int which, const uint32_t (&o)[16], int row, int col,
+                                                int columns) {
+  if (row >= p.m) return;
+  const int valid = min(columns, p.f - col);
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out[which]) + (static_cast<size_t>(row) * p.f + col) * 2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (8 * i < valid) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+}
+
 template <int kCta>
 __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
     gated_umma_kernel(const __grid_constant__ GatedParams p) {
@@ -86,22 +123,25 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
   const uint32_t lane = threadIdx.x & 31;
   const uint32_t cta_rank = (kCta == 2) ? ptx::cluster_ctarank() : 0u;
   const bool leader = cta_rank == 0;
-  const int first = static_cast<int>(blockIdx.x) / kCta;
-  const int stride = static_cast<int>(gridDim.x) / kCta;
+  const uint32_t ctas_per_tile = kCta == 2 ? 2u : static_cast<uint32_t>(p.split);
+  const uint32_t k_rank = (kCta == 1 && p.split > 1) ? ptx::cluster_ctarank() : 0u;  // which share of K is this CTA's
+  const int first = static_cast<int>(blockIdx.x / ctas_per_tile);
+  const int stride = static_cast<int>(gridDim.x / ctas_per_tile);
   const int tiles = p.m_tiles * p.n_tiles;
-  const int num_kb = (p.k + S::kBK - 1) / S::kBK;
+  const int all_kb = (p.k + S::kBK - 1) / S::kBK;
+  const int kb_base = kCta == 2 ? 0 : all_kb * static_cast<int>(k_rank) / p.split;
+  const int num_kb = kCta == 2 ? all_kb : all_kb * static_cast<int>(k_rank + 1) / p.split - kb_base;
 
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
-  const uint32_t ring_bytes = static_cast<uint32_t>(p.stages * p.stage_bytes);
-  const uint32_t staging_base = smem_base + ring_bytes;
-  const uint32_t bar_base = staging_base + S::kStagingBytes;
+  const uint32_t staging_base = smem_base + static_cast<uint32_t>(p.stages * p.stage_bytes);  // pair variant
+  const uint32_t bar_base = smem_base + static_cast<uint32_t>(p.bar_offset);
   auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (S::kMaxStages + s); };
   auto tmem_full_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + a); };
   auto tmem_empty_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + 2 + a); };
   volatile uint32_t* tmem_slot =
-      reinterpret_cast<volatile uint32_t*>(smem_gen + ring_bytes + S::kStagingBytes + 8 * (2 * S::kMaxStages + 4));
+      reinterpret_cast<volatile uint32_t*>(smem_gen + p.bar_offset + 8 * (2 * S::kMaxStages + 4));
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   // Groups of group_m row tiles are walked column-major, so tiles in flight together share rows of A and of the weights.
@@ -160,16 +200,17 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
         if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) break;
         if (ptx::elect_one()) {
           const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
-          const uint32_t b = a + S::kABytes;
+          const uint32_t b = a + static_cast<uint32_t>(p.a_bytes);
           if (leader) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
+          const int k0 = (kb_base + kb) * S::kBK;
           if constexpr (kCta == 2) {
             const uint32_t bar = ptx::mapa(full_bar(s), 0);
-            ptx::tma_load_2d_pair(a, &p.tm_a, bar, kb * S::kBK, row_a);
-            ptx::tma_load_2d_pair(b, tm_b, bar, kb * S::kBK, row_b);
+            ptx::tma_load_2d_pair(a, &p.tm_a, bar, k0, row_a);
+            ptx::tma_load_2d_pair(b, tm_b, bar, k0, row_b);
           } else {
-            ptx::tma_load_2d(b, &p.tm_gate, full_bar(s), kb * S::kBK, row_b);
-            ptx::tma_load_2d(b + b_bytes, &p.tm_up, full_bar(s), kb * S::kBK, row_b);
-            ptx::tma_load_2d(a, &p.tm_a, full_bar(s), kb * S::kBK, row_a);
+            ptx::tma_load_2d(b, &p.tm_gate, full_bar(s), k0, row_b);
+            ptx::tma_load_2d(b + b_bytes, &p.tm_up, full_bar(s), k0, row_b);
+            ptx::tma_load_2d(a, &p.tm_a, full_bar(s), k0, row_a);
           }
         }
         __syncwarp();
@@ -195,7 +236,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
       const uint32_t idesc =
           ptx::umma_idesc_f16_f32(S::kBM * kCta, 2 * p.width) | (p.bf16 ? ptx::kIdescBf16Inputs : 0u);
       const uint64_t a_desc0 = ptx::umma_desc_k_sw128(smem_base);
-      const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + S::kABytes);
+      const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + static_cast<uint32_t>(p.a_bytes));
       const uint64_t desc_stride = static_cast<uint64_t>(p.stage_bytes >> 4);
       const uint32_t stages = static_cast<uint32_t>(p.stages);
       uint32_t s = mine, ph = 0;
@@ -205,7 +246,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
         const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
         if (!bounded_wait_converged(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc, lane)) break;
         ptx::tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * S::kAccCols + mine * S::kChainCols;
+        const uint32_t d_tmem = tmem_base + acc * S::kAccCols + mine * kGatedChainCols;
         const int kb_first = kb;
         for (; kb < num_kb; kb += static_cast<int>(issuers)) {
           if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) break;
@@ -236,7 +277,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
         __syncwarp();
       }
     }
-  } else {
+  } else if (kCta == 2 || p.split == 1) {
     // ------------------------------------------------------------------ epilogue (warps 2..5)
     const uint32_t quad = warp & 3u;  // TMEM lanes [32 quad, 32 quad + 32) are this warp's to read
     const uint32_t lead_empty0 = (kCta == 2) ? ptx::mapa(tmem_empty_bar(0), 0) : tmem_empty_bar(0);
@@ -255,20 +296,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
       const bool rows_live = row0 < p.m;  // warp-uniform
       for (int c = 0; rows_live && c < p.width && col0 + c < p.f; c += 32) {
         uint32_t g[32], u[32];
-        ptx::tmem_ld_32x32(taddr + c, g);  // a narrow tile's last read runs into the neighbouring columns: not stored
-        ptx::tmem_ld_32x32(taddr + p.width + c, u);
-        ptx::tmem_ld_wait();
-        if (p.issuers == 2) {  // the second issuer's sums
-          uint32_t x[32];
-          ptx::tmem_ld_32x32(taddr + S::kChainCols + c, x);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int q = 0; q < 32; ++q) g[q] = __float_as_uint(__uint_as_float(g[q]) + __uint_as_float(x[q]));
-          ptx::tmem_ld_32x32(taddr + S::kChainCols + p.width + c, x);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(__uint_as_float(u[q]) + __uint_as_float(x[q]));
-        }
+        gated_load(p, taddr + c, g, u);  // a narrow tile's last read runs into the neighbouring columns: not stored
         // Writes 32 columns of output `which`, rounded once.
         auto store = [&](const uint32_t(&v)[32], int which) {
           uint32_t o[16];
@@ -296,15 +324,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
             }
             ++stores;
           } else {
-            const int row = row0 + static_cast<int>(lane);
-            const int valid = min(min(32, p.width - c), p.f - (col0 + c));  // a multiple of 8
-            if (row < p.m) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out[which]) +
-                                                    (static_cast<size_t>(row) * p.f + col0 + c) * 2);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (8 * i < valid) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            }
+            gated_store_row(p, which, o, row0 + static_cast<int>(lane), col0 + c, min(32, p.width - c));
           }
         };
         if (keep) {
@@ -321,6 +341,65 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
           ptx::mbar_arrive(tmem_empty_bar(acc));
         else
           ptx::mbar_arrive_cluster(lead_empty0 + 8u * acc);
+      }
+    }
+  }
+
+  if constexpr (kCta == 1) {
+    if (p.split > 1) {
+      // ---------------------------------------------------------------- a tile shared by a cluster: its epilogue
+      const uint32_t split = static_cast<uint32_t>(p.split);
+      const bool epilogue = warp >= 2 && warp < 6;
+      const uint32_t quad = warp & 3u;
+      const uint32_t row = quad * 32u + lane;
+      const uint32_t taddr = tmem_base + ((quad * 32u) << 16);
+      const int slice = p.width / p.split;  // columns of F that each CTA finishes, a multiple of 8
+      const uint32_t groups = static_cast<uint32_t>(slice) / 2u;  // of four floats: the slice's columns of both products
+      bool ready = false;
+      if (epilogue) {
+        ready = bounded_wait_warp(tmem_full_bar(0), 0, cta_abort, p.status, kFaultEpilogueWait, lane);
+        ptx::tc_fence_after();
+        ready = ready && static_cast<int>(quad * 32u) < p.m;
+      }
+      ptx::cluster_sync_all();  // every CTA's operands have been multiplied: the rings may be written over
+      if (ready) {
+        for (uint32_t to = 0; to < split; ++to) {
+          if (to == k_rank) continue;
+          const uint32_t there = ptx::mapa(smem_base, to);
+          for (int c = 0; c < slice; c += 32) {
+            uint32_t g[32], u[32];
+            gated_load(p, taddr + to * slice + c, g, u);
+            if (static_cast<int>(row) < p.m) {
+              const uint32_t slot = exchange_slot(k_rank, to), at = static_cast<uint32_t>(c) / 4u;
+              exchange_send(there, slot, groups, at, row, g, slice - c);
+              exchange_send(there, slot, groups, groups / 2u + at, row, u, slice - c);
+            }
+          }
+        }
+      }
+      ptx::cluster_sync_all();
+      if (ready) {
+        const int col0 = first * p.width + static_cast<int>(k_rank) * slice;
+        for (int c = 0; c < slice && col0 + c < p.f; c += 32) {
+          uint32_t g[32], u[32];
+          gated_load(p, taddr + k_rank * slice + c, g, u);
+          const uint32_t at = static_cast<uint32_t>(c) / 4u;
+          exchange_sum(smem_base, k_rank, split, groups, at, row, g, slice - c);
+          exchange_sum(smem_base, k_rank, split, groups, groups / 2u + at, row, u, slice - c);
+          auto store = [&](const uint32_t(&v)[32], int which) {
+            uint32_t o[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+              o[q] = ptx::pack_out2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]), p.bf16);
+            gated_store_row(p, which, o, static_cast<int>(row), col0 + c, min(32, slice - c));
+          };
+          if (p.out[1] != nullptr) {
+            store(g, 1);
+            store(u, 2);
+          }
+          gated_combine(p.act, g, u);
+          store(g, 0);
+        }
       }
     }
   }

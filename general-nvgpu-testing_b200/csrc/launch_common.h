@@ -16,7 +16,7 @@ inline bool overlap(const void* p, size_t pb, const void* q, size_t qb) {
   return p && q && a < b + qb && b < a + pb;
 }
 
-// How many CTAs (ctas = 1) or 2-CTA clusters (ctas = 2) of `kernel` the device holds at once, one per SM; the first call
+// How many clusters of `ctas` CTAs of `kernel` the device holds at once, one CTA per SM; the first call
 // on a device opts in to the large shared memory and asks.  `known` is the launcher's own table for this kernel.
 struct ResidentTable {
   std::mutex mutex;
@@ -32,14 +32,14 @@ int resident_grid(ResidentTable* known, Kernel kernel, DeviceCtx* ctx, int threa
     BEAM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes),
                   "cudaFuncSetAttribute(smem)");
     int fit = ctx->sm_count / ctas;
-    if (ctas == 2) {
+    if (ctas > 1) {
       cudaLaunchConfig_t probe = {};
-      probe.gridDim = dim3(static_cast<unsigned>(ctx->sm_count / 2 * 2), 1, 1);
+      probe.gridDim = dim3(static_cast<unsigned>(ctx->sm_count / ctas * ctas), 1, 1);
       probe.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
       probe.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
       attr[0].val.clusterDim.y = 1;
       attr[0].val.clusterDim.z = 1;
       probe.attrs = attr;

@@ -30,19 +30,27 @@ MxUnits lay_units(int rows, int k, int* grid) {
   return u;
 }
 
-// Columns per tile for M <= 128: B is read once whatever the width, so the width only deals out N.  64 or 128: a tile's scales
-// start at the first or the third of the four TMEM columns of a scale block, and a UMMA takes scales from even columns only
-// (a width of 32, which starts every other tile at an odd column, faulted with a misaligned address).
-int narrow_width(int n, int sm_count) { return ceil_div(n, 64) <= sm_count ? 64 : 128; }
+// Tiles for M <= 128.  B is read once whatever the tiles, so they only deal out N and K.  64 or 128 columns: a tile's scales start at
+// the first or the third of the four TMEM columns of a scale block, and a UMMA takes scales from even columns only (a width
+// of 32, which starts every other tile at an odd column, faulted with a misaligned address).  64 wherever that is one wave.
+// Where SMs are left over and K is long, clusters of 2 or 4 CTAs share a tile's contraction.  Measured, one row, us with
+// 1 / 2 / 4 CTAs: N = 2072, K = 8192 9.2 / 7.3 / 7.2; 1024, 4096 6.1 / 5.9 / 6.1; 4096, 4096 6.4 / 6.1; 2048, 2048 5.0 / 5.2 / 5.8; and
+// with 128 columns 9.9 / 8.1 / 7.3, 6.9 / 6.5 / 6.3, 7.3 / 6.7, 5.6 / 5.6 / 5.9.
+struct NarrowPlan {
+  int width, split;
+};
+NarrowPlan narrow_plan(int n, int k, const int (&fit)[3]) {
+  const int tiles = ceil_div(n, 64), stages = ceil_div(k, 256);
+  if (tiles > fit[0]) return {128, 1};
+  if (stages >= 32 && tiles <= fit[2]) return {64, 4};
+  if (stages >= 16 && tiles <= fit[1]) return {64, 2};
+  return {64, 1};
+}
 
 template <int kCta>
-int launch_instance(DeviceCtx* ctx, const void* A, const void* sa, const void* B, const void* sb, void* C, int m, int n,
-                    int k, int bf16, cudaStream_t stream) {
+int launch_instance(DeviceCtx* ctx, const NarrowPlan& plan, int resident, const void* A, const void* sa, const void* B,
+                    const void* sb, void* C, int m, int n, int k, int bf16, cudaStream_t stream) {
   using S = MxShape<kCta>;
-  static ResidentTable table;
-  int resident = 0;
-  int st = resident_grid(&table, mxfp4_umma_kernel<kCta>, ctx, S::kThreads, S::kSmemLimit, kCta, &resident);
-  if (st != BEAM_OK) return st;
   MxGemmParams p = {};
   p.c = C;
   p.m = m;
@@ -50,25 +58,36 @@ int launch_instance(DeviceCtx* ctx, const void* A, const void* sa, const void* B
   p.k = k;
   p.bf16 = bf16;
   p.status = ctx->status_word;
-  p.width = kCta == 2 ? S::kMaxWidth : narrow_width(n, resident);
+  p.width = plan.width;
+  p.split = plan.split;
   p.a_rows = kCta == 2 ? 128 : (m + 7) / 8 * 8;
-  p.stage_bytes = S::kABytes + p.width / kCta * 128 + S::kScaleBytes;
-  p.stages = S::kRingBytes / p.stage_bytes;
-  if (p.stages > S::kMaxStages) p.stages = S::kMaxStages;
+  p.a_bytes = p.a_rows * 128;
+  p.stage_bytes = p.a_bytes + p.width / kCta * 128 + S::kScaleBytes;
   p.m_tiles = ceil_div(m, 128 * kCta);
   p.n_tiles = ceil_div(n, p.width);
   p.group_m = 8;
-  const uint64_t words = 64ull * ceil_div(k, 128);
-  st = encode_tmap_2d_u8(&p.tm_a, A, m, k / 2, static_cast<uint32_t>(p.a_rows), 128);
-  if (st == BEAM_OK) st = encode_tmap_2d_u8(&p.tm_b, B, n, k / 2, static_cast<uint32_t>(p.width / kCta), 128);
-  if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sa, sa, ceil_div(m, 128), words, 1, 128);
-  if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sb, sb, ceil_div(n, 128), words, 2, 128);
-  if (st == BEAM_OK && kCta == 2) st = encode_tmap_2d(&p.tm_c, C, 2, m, n, n, 32, 64, true);
-  if (st != BEAM_OK) return st;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
   const int clusters = tiles < resident ? static_cast<int>(tiles) : resident;
-  const int smem = p.stages * p.stage_bytes + S::kStagingBytes + S::kBarBytes;
-  return launch_dependent(mxfp4_umma_kernel<kCta>, clusters * kCta, S::kThreads, smem, kCta, stream,
+  // Two issuers where a CTA has one tile, whose two accumulators take the place of the next tile's; every CTA must have a
+  // stage for each.
+  p.issuers = kCta == 1 && tiles <= resident && ceil_div(k, S::kBK) >= 2 * p.split ? 2 : 1;
+  // A UMMA reads 128 rows of A whether they were loaded or not: behind the last stage there is room for them.
+  const int a_slack = S::kABytes - p.a_bytes;
+  p.stages = (S::kRingBytes - a_slack) / p.stage_bytes;
+  if (p.stages > S::kMaxStages) p.stages = S::kMaxStages;
+  if (p.issuers == 2) p.stages &= ~1;
+  const int exchange = (p.split - 1) * (p.width / p.split) * 128 * 4;  // what the others of a cluster send
+  p.bar_offset = p.stages * p.stage_bytes + a_slack + S::kStagingBytes;
+  if (p.bar_offset < exchange) p.bar_offset = exchange;
+  const uint64_t words = 64ull * ceil_div(k, 128);
+  int st = encode_tmap_2d_u8(&p.tm_a, A, m, k / 2, static_cast<uint32_t>(p.a_rows), 128);
+  if (st == BEAM_OK) st = encode_tmap_2d_u8(&p.tm_b, B, n, k / 2, static_cast<uint32_t>(p.width / kCta), 128);
+  if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sa, sa, ceil_div(m, 128), words, 1, 128);
+  if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sb, sb, ceil_div(n, 128), words, S::kScaleBlocksB, 128);
+  if (st == BEAM_OK && kCta == 2) st = encode_tmap_2d(&p.tm_c, C, 2, m, n, n, 32, 64, true);
+  if (st != BEAM_OK) return st;
+  const int ctas = kCta * p.split;
+  return launch_dependent(mxfp4_umma_kernel<kCta>, clusters * ctas, S::kThreads, p.bar_offset + S::kBarBytes, ctas, stream,
                           "cudaLaunchKernelEx(mxfp4_umma)", p);
 }
 
@@ -136,8 +155,19 @@ int launch_mxfp4_gemmrc(const void* A, const void* a_scales, const void* B, cons
     return BEAM_ERR_INVALID_ARG;
   DeviceCtx* ctx = current_device_ctx(&st);
   if (!ctx) return st;
-  return m <= 128 ? launch_instance<1>(ctx, A, a_scales, B, b_scales, C, m, n, k, bf16, stream)
-                  : launch_instance<2>(ctx, A, a_scales, B, b_scales, C, m, n, k, bf16, stream);
+  static ResidentTable table[4];
+  int fit[3], pairs = 0;  // single CTAs; clusters of 2 and 4 CTAs that share a contraction; pairs
+  if (m > 128) {
+    st = resident_grid(&table[3], mxfp4_umma_kernel<2>, ctx, MxShape<2>::kThreads, MxShape<2>::kSmemLimit, 2, &pairs);
+    if (st != BEAM_OK) return st;
+    return launch_instance<2>(ctx, {MxShape<2>::kMaxWidth, 1}, pairs, A, a_scales, B, b_scales, C, m, n, k, bf16, stream);
+  }
+  for (int i = 0; i < 3; ++i) {
+    st = resident_grid(&table[i], mxfp4_umma_kernel<1>, ctx, MxShape<1>::kThreads, MxShape<1>::kSmemLimit, 1 << i, &fit[i]);
+    if (st != BEAM_OK) return st;
+  }
+  const NarrowPlan plan = narrow_plan(n, k, fit);
+  return launch_instance<1>(ctx, plan, fit[plan.split / 2], A, a_scales, B, b_scales, C, m, n, k, bf16, stream);
 }
 
 }  // namespace beam

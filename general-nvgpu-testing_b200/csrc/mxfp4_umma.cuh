@@ -150,18 +150,23 @@ static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint
 // C[M, N] = A B^T: 4-bit UMMAs (K = 64) with block scales, fp32 accumulation, one rounding to fp16 or bf16.
 //
 // A stage of the ring is 256 elements of K: 128 bytes per row, laid out by TMA with the 128-byte swizzle like any K-major
-// operand, and 3 KB of scale blocks (one row block for A, two for B) that a second copy brings as they are.  Per stage
-// the issuing thread copies six scale blocks into TMEM and issues four UMMAs; copies and UMMAs of one thread execute in
-// order, so nothing else separates them; two sets of scale columns alternate.
+// operand, and 1 KB of scale blocks per 128 rows that a second copy brings as they are.  Per stage the issuing warp copies
+// the scale blocks into TMEM and issues four UMMAs; copies and UMMAs of one thread execute in order, so nothing else
+// separates them; two sets of scale columns alternate.
 //
 //   kCta = 2   256 x 256 tiles on a pair.  B's scales of all 256 columns are needed in both CTAs' TMEM, so both load them.
 //              Two accumulators of 256 columns and the scales do not fit into 512 columns, so the accumulators overlap
 //              by 64 columns: the epilogue of a tile drains that part first and hands it back, after which the next
 //              tile's UMMAs may start in the other accumulator while the rest is drained.
-//   kCta = 1   M <= 128, bound by reading B: 128 rows x 64 or 128 columns (a tile's scales start at an even TMEM column),
-//              whichever deals N to the SMs; only existing rows of A are loaded.
+//              What bounds it at 8192^3 (177 us, 6.2 PFLOP/s): the tensor pipe is active 69 % of the cycles; copies alone
+//              (no UMMA, no scales) take 150 us, UMMAs without the scale copies 6 % less than with them, and each tile
+//              begins with a wait for the hand-back of about 1 us.  A sixth stage in place of the second store buffer
+//              took 190 us to 184; scales copied one stage ahead changed nothing (221 against 220).
+//   kCta = 1   M <= 128, bound by reading B: 128 rows x 64 or 128 columns (see narrow_plan() in mxfp4_launch.cu).  Only existing
+//              rows of A are loaded, two issuers take turns at the stages, and clusters may share a contraction, all
+//              as in gated_umma.cuh.
 //
-// Roles: warp 0 loads A and its scales, warp 6 B and its scales, warp 1 issues, warps 2..5 are the epilogue.
+// Roles: warp 0 loads A and its scales, warp 6 B and its scales, warps 1 and 7 issue, warps 2..5 are the epilogue.
 struct MxGemmParams {
   CUtensorMap tm_a;   // packed A [M, K / 2 bytes], box (rows per CTA) x 128
   CUtensorMap tm_b;   // packed B [N, K / 2 bytes], box (width / kCta) x 128
@@ -173,6 +178,10 @@ struct MxGemmParams {
   int width;          // columns per tile
   int a_rows;         // rows of A that a CTA loads
   int stages, stage_bytes;
+  int a_bytes;        // of a stage: B begins there, the scales behind B
+  int bar_offset;     // the barriers' place in shared memory, behind the ring and what else takes its place
+  int issuers;        // warps that issue UMMAs: 1, or 2 that take turns at the stages, an accumulator and scale columns each
+  int split;          // single CTAs: a cluster of this many CTAs shares each tile's contraction
   int m_tiles, n_tiles, group_m;
   int bf16;
   int* status;
@@ -182,20 +191,53 @@ template <int kCta>
 struct MxShape {
   static constexpr int kBK = 256;  // elements of K per stage
   static constexpr int kABytes = 128 * 128;
-  static constexpr int kScaleBytes = 3 * 1024;
-  static constexpr int kMaxStages = 8;
-  static constexpr int kThreads = 224;
+  static constexpr int kScaleBlocksB = kCta;  // row blocks of B's scales per tile
+  static constexpr int kScaleBytes = (1 + kScaleBlocksB) * 1024;
+  static constexpr int kMaxStages = 16;
+  static constexpr int kThreads = 256;  // warp 7: the second issuer
   static constexpr int kMaxWidth = kCta == 2 ? 256 : 128;
   static constexpr int kAccStep = kCta == 2 ? 192 : 128;  // TMEM columns from one accumulator to the other
-  static constexpr int kScaleCols = kAccStep + kMaxWidth;  // first column of the scales: two sets of 2 x (4 + 8)
+  static constexpr int kScaleCols = kAccStep + kMaxWidth;  // first column of the scales
+  static constexpr int kScaleHalf = 4 + 4 * kScaleBlocksB;  // columns of 128 elements of K
+  static constexpr int kScaleSet = 2 * kScaleHalf;          // ... of a stage; an issuer alternates between two sets
   static constexpr int kBufsPerWarp = 1;
   static constexpr int kStagingBytes = kCta == 2 ? 4 * kBufsPerWarp * 4096 : 0;
-  static constexpr int kBarBytes = 256;
+  static constexpr int kBarBytes = 512;
   static constexpr int kSmemLimit = 232448;
   static constexpr int kRingBytes = kSmemLimit - kStagingBytes - kBarBytes;
-  static_assert(kScaleCols + 2 * 24 <= 512, "accumulators and scales share 512 columns");
+  static_assert(kScaleCols + (3 - kCta) * 2 * kScaleSet <= 512, "accumulators and scales share 512 columns");
   static_assert((2 * kMaxStages + 4) * 8 + 8 <= kBarBytes, "barrier block too small");
 };
+
+// 32 columns of a single CTA's tile from TMEM, the two issuers' sums added where there are two.
+__device__ __forceinline__ void mx_load(const MxGemmParams& p, uint32_t taddr, uint32_t (&v)[32]) {
+  ptx::tmem_ld_32x32(taddr, v);
+  ptx::tmem_ld_wait();
+  if (p.issuers == 2) {
+    uint32_t x[32];
+    ptx::tmem_ld_32x32(taddr + MxShape<1>::kAccStep, x);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(__uint_as_float(v[q]) + __uint_as_float(x[q]));
+  }
+}
+
+// One row's share of up to 32 columns, rounded, straight to C; columns is a multiple of 8, as is N.
+__device__ __forceinline__ void mx_store_row(const MxGemmParams& p, const uint32_t (&v)[32], int row, int col, int columns) {
+  if (row >= p.m) return;
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.c) + (static_cast<size_t>(row) * p.n + col) * 2);
+  const int valid = min(columns, p.n - col);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (8 * i < valid) {
+      uint32_t o[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        o[q] = ptx::pack_out2(__uint_as_float(v[8 * i + 2 * q]), __uint_as_float(v[8 * i + 2 * q + 1]), p.bf16);
+      dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
 
 template <int kCta>
 __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(const __grid_constant__ MxGemmParams p) {
@@ -205,22 +247,26 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
   const uint32_t lane = threadIdx.x & 31;
   const int cta_rank = (kCta == 2) ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   const bool leader = cta_rank == 0;
-  const int first = static_cast<int>(blockIdx.x) / kCta;
-  const int stride = static_cast<int>(gridDim.x) / kCta;
+  const int ctas_per_tile = kCta == 2 ? 2 : p.split;
+  const uint32_t k_rank = (kCta == 1 && p.split > 1) ? ptx::cluster_ctarank() : 0u;  // which share of K is this CTA's
+  const int first = static_cast<int>(blockIdx.x) / ctas_per_tile;
+  const int stride = static_cast<int>(gridDim.x) / ctas_per_tile;
   const int tiles = p.m_tiles * p.n_tiles;
-  const int num_kb = (p.k + S::kBK - 1) / S::kBK;
+  const int all_kb = (p.k + S::kBK - 1) / S::kBK;
+  const int kb_base = kCta == 2 ? 0 : all_kb * static_cast<int>(k_rank) / p.split;
+  const int num_kb = kCta == 2 ? all_kb : all_kb * static_cast<int>(k_rank + 1) / p.split - kb_base;
 
   const uint32_t smem_base = ptx::smem_u32(smem_tiles);
-  const uint32_t ring_bytes = static_cast<uint32_t>(p.stages * p.stage_bytes);
+  const uint32_t a_bytes = static_cast<uint32_t>(p.a_bytes);
   const uint32_t b_bytes = static_cast<uint32_t>(p.width / kCta) * 128u;
-  const uint32_t staging_base = smem_base + ring_bytes;
-  const uint32_t bar_base = staging_base + S::kStagingBytes;
+  const uint32_t staging_base = smem_base + static_cast<uint32_t>(p.stages * p.stage_bytes);  // pair variant
+  const uint32_t bar_base = smem_base + static_cast<uint32_t>(p.bar_offset);
   auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (S::kMaxStages + s); };
   auto tmem_full_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + a); };
   auto tmem_empty_bar = [&](uint32_t a) { return bar_base + 8u * (2 * S::kMaxStages + 2 + a); };
   volatile uint32_t* tmem_slot =
-      reinterpret_cast<volatile uint32_t*>(smem_tiles + ring_bytes + S::kStagingBytes + 8 * (2 * S::kMaxStages + 4));
+      reinterpret_cast<volatile uint32_t*>(smem_tiles + p.bar_offset + 8 * (2 * S::kMaxStages + 4));
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   auto tile_at = [&](int t, int& mt, int& nt) {
@@ -239,7 +285,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
       ptx::mbar_init(empty_bar(s), 1);
     }
     for (uint32_t a = 0; a < 2; ++a) {
-      ptx::mbar_init(tmem_full_bar(a), 1);
+      ptx::mbar_init(tmem_full_bar(a), static_cast<uint32_t>(p.issuers));
       ptx::mbar_init(tmem_empty_bar(a), 4 * kCta);
     }
     *cta_abort = 0;
@@ -281,26 +327,27 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         }
         if (ptx::elect_one()) {
           const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
-          const uint32_t b = a + S::kABytes;
+          const uint32_t b = a + a_bytes;
           const uint32_t sf = b + b_bytes;
+          const int x = (kb_base + kb) * 128;
           // A's producer arms the barrier with the whole stage; B's bytes may land before that (see grad_umma.cuh).
           if (left && leader) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
           if constexpr (kCta == 2) {
             const uint32_t bar = ptx::mapa(full_bar(s), 0);
             if (left) {
-              ptx::tma_load_2d_pair(a, &p.tm_a, bar, kb * 128, block_a * 128);
-              ptx::tma_load_2d_pair(sf, &p.tm_sa, bar, kb * 128, block_a);
+              ptx::tma_load_2d_pair(a, &p.tm_a, bar, x, block_a * 128);
+              ptx::tma_load_2d_pair(sf, &p.tm_sa, bar, x, block_a);
             } else {
-              ptx::tma_load_2d_pair(b, &p.tm_b, bar, kb * 128, col + cta_rank * 128);
-              ptx::tma_load_2d_pair(sf + 1024u, &p.tm_sb, bar, kb * 128, col >> 7);
+              ptx::tma_load_2d_pair(b, &p.tm_b, bar, x, col + cta_rank * 128);
+              ptx::tma_load_2d_pair(sf + 1024u, &p.tm_sb, bar, x, col >> 7);
             }
           } else {
             if (left) {
-              ptx::tma_load_2d(a, &p.tm_a, full_bar(s), kb * 128, block_a * 128);
-              ptx::tma_load_2d(sf, &p.tm_sa, full_bar(s), kb * 128, block_a);
+              ptx::tma_load_2d(a, &p.tm_a, full_bar(s), x, block_a * 128);
+              ptx::tma_load_2d(sf, &p.tm_sa, full_bar(s), x, block_a);
             } else {
-              ptx::tma_load_2d(b, &p.tm_b, full_bar(s), kb * 128, col);
-              ptx::tma_load_2d(sf + 1024u, &p.tm_sb, full_bar(s), kb * 128, col >> 7);
+              ptx::tma_load_2d(b, &p.tm_b, full_bar(s), x, col);
+              ptx::tma_load_2d(sf + 1024u, &p.tm_sb, full_bar(s), x, col >> 7);
             }
           }
         }
@@ -311,22 +358,23 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         }
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (leader) {
+  } else if (warp == 1 || warp == 7) {
+    // ------------------------------------------------------------------ MMA issuers (two: see gated_umma.cuh)
+    const uint32_t issuers = static_cast<uint32_t>(p.issuers);
+    const uint32_t mine = warp == 1 ? 0u : 1u;
+    if (leader && mine < issuers) {
       const uint32_t idesc0 = ptx::umma_idesc_mxf4(128 * kCta, p.width, 0);
       const uint32_t idesc2 = ptx::umma_idesc_mxf4(128 * kCta, p.width, 2);
       const uint64_t a_desc0 = ptx::umma_desc_k_sw128(smem_base);
-      const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + S::kABytes);
-      const uint64_t sf_desc0 = ptx::umma_desc_scales(smem_base + S::kABytes + b_bytes);
+      const uint64_t b_desc0 = ptx::umma_desc_k_sw128(smem_base + a_bytes);
+      const uint64_t sf_desc0 = ptx::umma_desc_scales(smem_base + a_bytes + b_bytes);
       const uint64_t desc_stride = static_cast<uint64_t>(p.stage_bytes >> 4);
       const uint32_t stages = static_cast<uint32_t>(p.stages);
-      const int steps = (p.k + 63) / 64;  // UMMAs per tile
-      const uint32_t scale_cols = tmem_base + S::kScaleCols;
-
-      uint32_t s = 0, ph = 0, set = 0;
-      bool alive = true;
-      for (int t = first, j = 0; alive && t < tiles; t += stride, ++j) {
+      const int steps = (p.k + 63) / 64 - kb_base * 4;  // UMMAs of a tile from this CTA's first k-block on
+      const uint32_t scale_cols = tmem_base + S::kScaleCols + mine * 2u * S::kScaleSet;
+      uint32_t s = mine, ph = 0, set = 0;
+      int kb = static_cast<int>(mine);
+      for (int t = first, j = 0; t < tiles; t += stride, ++j) {
         int mt, nt;
         tile_at(t, mt, nt);
         const uint32_t acc = static_cast<uint32_t>(j) & 1u;
@@ -342,30 +390,31 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         }
         if (!drained) break;
         ptx::tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * S::kAccStep;
+        const uint32_t d_tmem = tmem_base + (acc + mine) * S::kAccStep;  // two issuers: one tile only, acc 0
         // a tile that starts inside a block of 128 columns starts inside that block's four TMEM columns
         const uint32_t sfb_shift = static_cast<uint32_t>(((nt * p.width) & 127) >> 5);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) {
-            alive = false;
-            break;
-          }
+        const int kb_first = kb;
+        for (; kb < num_kb; kb += static_cast<int>(issuers)) {
+          if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) break;
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
             const uint64_t a = a_desc0 + s * desc_stride, b = b_desc0 + s * desc_stride, sf = sf_desc0 + s * desc_stride;
-            const uint32_t sfa = scale_cols + set * 24u, sfb = sfa + 4u;
+            const uint32_t sfa = scale_cols + set * S::kScaleSet, sfb = sfa + 4u;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
-              ptx::tmem_cp_scales<kCta>(sfa + h * 12u, sf + h * (512 >> 4));
-              ptx::tmem_cp_scales<kCta>(sfb + h * 12u, sf + ((1024 + h * 512) >> 4));
-              ptx::tmem_cp_scales<kCta>(sfb + h * 12u + 4u, sf + ((2048 + h * 512) >> 4));
+              ptx::tmem_cp_scales<kCta>(sfa + h * S::kScaleHalf, sf + h * (512 >> 4));
+#pragma unroll
+              for (uint32_t i = 0; i < S::kScaleBlocksB; ++i)
+                ptx::tmem_cp_scales<kCta>(sfb + h * S::kScaleHalf + 4u * i, sf + ((1024 * (1 + i) + h * 512) >> 4));
             }
             const int live = steps - kb * 4;  // steps past K are left out: their scales may lie outside the matrix
             const uint32_t from = sfb + sfb_shift;
-            ptx::umma_mxf4<kCta>(d_tmem, a, b, idesc0, sfa, from, kb > 0 ? 1u : 0u);
+            ptx::umma_mxf4<kCta>(d_tmem, a, b, idesc0, sfa, from, kb > kb_first ? 1u : 0u);
             if (live > 1) ptx::umma_mxf4<kCta>(d_tmem, a + 2, b + 2, idesc2, sfa, from, 1u);
-            if (live > 2) ptx::umma_mxf4<kCta>(d_tmem, a + 4, b + 4, idesc0, sfa + 12u, from + 12u, 1u);
-            if (live > 3) ptx::umma_mxf4<kCta>(d_tmem, a + 6, b + 6, idesc2, sfa + 12u, from + 12u, 1u);
+            if (live > 2)
+              ptx::umma_mxf4<kCta>(d_tmem, a + 4, b + 4, idesc0, sfa + S::kScaleHalf, from + S::kScaleHalf, 1u);
+            if (live > 3)
+              ptx::umma_mxf4<kCta>(d_tmem, a + 6, b + 6, idesc2, sfa + S::kScaleHalf, from + S::kScaleHalf, 1u);
             if constexpr (kCta == 1)
               ptx::umma_commit<1>(empty_bar(s));
             else
@@ -373,12 +422,15 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
           }
           __syncwarp();
           set ^= 1u;
-          if (++s == stages) {
-            s = 0;
+          s += issuers;
+          if (s >= stages) {
+            s -= stages;
             ph ^= 1u;
           }
         }
-        if (alive && ptx::elect_one()) {
+        if (kb < num_kb) break;  // a wait ran out
+        kb -= num_kb;
+        if (ptx::elect_one()) {
           if constexpr (kCta == 1)
             ptx::umma_commit<1>(tmem_full_bar(acc));
           else
@@ -387,7 +439,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         __syncwarp();
       }
     }
-  } else {
+  } else if (kCta == 2 || p.split == 1) {
     // ------------------------------------------------------------------ epilogue (warps 2..5)
     const uint32_t quad = warp & 3u;
     const uint32_t lead_empty0 = (kCta == 2) ? ptx::mapa(tmem_empty_bar(0), 0) : tmem_empty_bar(0);
@@ -445,27 +497,53 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         const int row = row0 + static_cast<int>(lane);
         for (int c = 0; row0 < p.m && c < p.width && col0 + c < p.n; c += 32) {
           uint32_t v[32];
-          ptx::tmem_ld_32x32(taddr + c, v);
-          ptx::tmem_ld_wait();
-          if (row < p.m) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.c) +
-                                                  (static_cast<size_t>(row) * p.n + col0 + c) * 2);
-            const int valid = min(32, p.n - (col0 + c));  // a multiple of 8
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (8 * i < valid) {
-                uint32_t o[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  o[q] = ptx::pack_out2(__uint_as_float(v[8 * i + 2 * q]), __uint_as_float(v[8 * i + 2 * q + 1]), p.bf16);
-                dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
-              }
-            }
-          }
+          mx_load(p, taddr + c, v);
+          mx_store_row(p, v, row, col0 + c, 32);
         }
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(tmem_empty_bar(acc));
+      }
+    }
+  }
+
+  if constexpr (kCta == 1) {
+    if (p.split > 1) {
+      // ---------------------------------------------------------------- a tile shared by a cluster: its epilogue
+      const uint32_t split = static_cast<uint32_t>(p.split);
+      const uint32_t quad = warp & 3u;
+      const uint32_t row = quad * 32u + lane;
+      const uint32_t taddr = tmem_base + ((quad * 32u) << 16);
+      const int slice = p.width / p.split;  // columns that each CTA finishes, a multiple of 8
+      const uint32_t groups = static_cast<uint32_t>(slice) / 4u;
+      bool ready = false;
+      if (warp >= 2 && warp < 6) {
+        ready = bounded_wait_warp(tmem_full_bar(0), 0, cta_abort, p.status, kFaultEpilogueWait, lane);
+        ptx::tc_fence_after();
+        ready = ready && static_cast<int>(quad * 32u) < p.m;
+      }
+      ptx::cluster_sync_all();  // every CTA's operands have been multiplied: the rings may be written over
+      if (ready) {
+        for (uint32_t to = 0; to < split; ++to) {
+          if (to == k_rank) continue;
+          const uint32_t there = ptx::mapa(smem_base, to);
+          for (int c = 0; c < slice; c += 32) {
+            uint32_t v[32];
+            mx_load(p, taddr + to * slice + c, v);
+            if (static_cast<int>(row) < p.m)
+              exchange_send(there, exchange_slot(k_rank, to), groups, static_cast<uint32_t>(c) / 4u, row, v, slice - c);
+          }
+        }
+      }
+      ptx::cluster_sync_all();
+      if (ready) {
+        const int col0 = first * p.width + static_cast<int>(k_rank) * slice;
+        for (int c = 0; c < slice && col0 + c < p.n; c += 32) {
+          uint32_t v[32];
+          mx_load(p, taddr + k_rank * slice + c, v);
+          exchange_sum(smem_base, k_rank, split, groups, static_cast<uint32_t>(c) / 4u, row, v, slice - c);
+          mx_store_row(p, v, static_cast<int>(row), col0 + c, min(32, slice - c));
+        }
       }
     }
   }

@@ -92,6 +92,49 @@ __device__ __forceinline__ bool bounded_wait_converged(uint32_t bar, uint32_t pa
   return ok;
 }
 
+// ---- joining the sums of a contraction that the CTAs of a cluster have split among them
+// Every CTA holds the sums over its own share of K, fp32 in TMEM.  Each finishes one slice of the columns: it sends the others'
+// slices into their shared memory (their rings are idle by then) and adds what arrives to its own.  What one source sends is
+// [groups of 4 columns][128 rows], so consecutive lanes write consecutive 16 bytes.  `valid` of the 32 columns are moved, a
+// multiple of 4.
+__device__ __forceinline__ uint32_t exchange_slot(uint32_t from, uint32_t to) { return from < to ? from : from - 1; }
+__device__ __forceinline__ void exchange_send(uint32_t cluster_base, uint32_t slot, uint32_t groups, uint32_t group,
+                                              uint32_t row, const uint32_t (&v)[32], int valid) {
+  const uint32_t at = cluster_base + ((slot * groups + group) * 128u + row) * 16u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (4 * i < valid)
+      ptx::st_cluster_f32x4(at + i * 2048u, __uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                            __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+}
+// v = the sum over all ranks, in their order; `v` comes in as this rank's own share.
+__device__ __forceinline__ void exchange_sum(uint32_t base, uint32_t rank, uint32_t ranks, uint32_t groups, uint32_t group,
+                                             uint32_t row, uint32_t (&v)[32], int valid) {
+  float sum[32];
+#pragma unroll
+  for (int q = 0; q < 32; ++q) sum[q] = 0.f;
+  for (uint32_t from = 0; from < ranks; ++from) {
+    if (from == rank) {
+#pragma unroll
+      for (int q = 0; q < 32; ++q) sum[q] += __uint_as_float(v[q]);
+    } else {
+      const uint32_t at = base + ((exchange_slot(from, rank) * groups + group) * 128u + row) * 16u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (4 * i < valid) {
+          const float4 x = ptx::ld_shared_f32x4(at + i * 2048u);
+          sum[4 * i] += x.x;
+          sum[4 * i + 1] += x.y;
+          sum[4 * i + 2] += x.z;
+          sum[4 * i + 3] += x.w;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(sum[q]);
+}
+
 // After an abort, give asynchronous work this CTA already issued (TMA copies into its shared
 // memory, UMMAs into its TMEM) time to land before shared memory and TMEM are released.
 __device__ __forceinline__ void abort_drain_delay() {

@@ -209,7 +209,8 @@ def test_slopes_against_differences(act):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,f,k", [(1, 8, 8), (1, 1504, 264), (2, 8, 1000), (7, 24, 72), (8, 2368, 64), (17, 1192, 200),
-                                   (64, 128, 512), (77, 5464, 136), (127, 3000, 8), (128, 1184, 64)])
+                                   (64, 128, 512), (77, 5464, 136), (127, 3000, 8), (128, 1184, 64),
+                                   (1, 1000, 3080), (33, 1192, 4104), (128, 2360, 2056), (100, 8, 8200)])
 def test_gated_few_rows(beam, healthy, dtype, m, f, k):
     """Up to 128 rows: widths from 8 to 40 columns per tile, ragged in every direction; nothing written past c."""
     a, bg, bu = gated_inputs(m, f, k, dtype, m + f)

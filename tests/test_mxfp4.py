@@ -211,7 +211,8 @@ def test_infinities_and_nan_stay_in_their_block(beam, healthy, dtype):
 @pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
 @pytest.mark.parametrize("m,n,k", [(1, 8, 32), (1, 4736, 256), (2, 128, 64), (7, 200, 96), (16, 1192, 160), (77, 5464, 128),
                                    (128, 4744, 1056), (128, 264, 4096), (129, 8, 32), (200, 264, 96), (256, 256, 256),
-                                   (300, 1000, 1376), (513, 776, 544), (1024, 2048, 2048), (2304, 2560, 512)])
+                                   (300, 1000, 1376), (513, 776, 544), (1024, 2048, 2048), (2304, 2560, 512),
+                                   (5, 20008, 320), (33, 2072, 8224), (128, 4100 // 4 * 8, 4128)])
 def test_product(beam, healthy, dtype, m, n, k):
     a, b = matrix(m, k, dtype, m + k), matrix(n, k, dtype, n, k ** -0.5)
     a64, b64 = round64(a)[0], round64(b)[0]
