@@ -113,7 +113,9 @@ def _load():
     L.beam_gated_gemmrc_backward_workspace_bytes.restype = sz
     L.beam_gated_gemmrc_backward_workspace_bytes.argtypes = [i, i, i]
     L.beam_gated_gemmrc_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, vp, sz, vp]
-    L.beam_gemmrc_backward.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp]
+    L.beam_gemmrc_backward_workspace_bytes.restype = sz
+    L.beam_gemmrc_backward_workspace_bytes.argtypes = [i, i, i]
+    L.beam_gemmrc_backward.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
     L.beam_mxfp4_quantize.argtypes = [vp, vp, vp, i, i, i, vp]
     L.beam_mxfp4_dequantize.argtypes = [vp, vp, vp, i, i, i, vp]
     L.beam_mxfp4_gemmrc.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp]
@@ -438,6 +440,15 @@ def _call(fn_name, device, *args):
         _raise(st, fn_name)
 
 
+def _sized(fn_name, device, *sizes):
+    """A workspace size, which goes by the device."""
+    fn = getattr(_lib or _load(), fn_name)
+    if torch.cuda.current_device() == device.index:
+        return fn(*sizes)
+    with torch.cuda.device(device):
+        return fn(*sizes)
+
+
 def gated_gemmrc(a, b_gate, b_up, c, activation="silu", gate=None, up=None):
     """c[M,F] = act(a @ b_gate.T) * (a @ b_up.T) in one kernel: the gated half of a feed-forward block.
 
@@ -466,7 +477,7 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
 
     dc, gate and up are [M,F]; gate and up are what the forward call kept.  The gradients wanted are given as tensors
     (at least one) and overwritten.  dg and du are rounded to the operands' type between the two steps; they are
-    held in scratch of 4 M F bytes from torch's allocator."""
+    held in scratch of 4 M F bytes (and more for short batches) from torch's allocator."""
     act = _activation(activation)
     m, k = _check_first("a", a, _HALF_TYPES)
     dtype, device, f = a.dtype, a.device, _rows(b_gate)
@@ -483,7 +494,7 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
         _check_matrix("db_gate", db_gate, (f, k), dtype, device)
     if db_up is not None:
         _check_matrix("db_up", db_up, (f, k), dtype, device)
-    nbytes = (_lib or _load()).beam_gated_gemmrc_backward_workspace_bytes(m, f, k)
+    nbytes = _sized("beam_gated_gemmrc_backward_workspace_bytes", device, m, f, k)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _call("beam_gated_gemmrc_backward", device, dc.data_ptr(), a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(),
           gate.data_ptr(), up.data_ptr(), _ptr(da), _ptr(db_gate), _ptr(db_up), m, f, k, act, _half_flags(a),
@@ -503,8 +514,10 @@ def gemmrc_backward(dc, a, b, da=None, db=None):
         _check_matrix("da", da, (m, k), dtype, device)
     if db is not None:
         _check_matrix("db", db, (n, k), dtype, device)
+    nbytes = _sized("beam_gemmrc_backward_workspace_bytes", device, m, n, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _call("beam_gemmrc_backward", device, dc.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(da), _ptr(db), m, n, k,
-          _half_flags(a))
+          _half_flags(a), _ptr(ws), nbytes)
 
 
 def _mxfp4_scales_shape(rows, k):

@@ -192,7 +192,7 @@ int beam_gated_gemmrc(const void* A, const void* B_gate, const void* B_up, void*
 }
 
 size_t beam_gated_gemmrc_backward_workspace_bytes(int m, int f, int k) {
-  return k > 0 ? gated_backward_workspace_bytes(m, f) : 0;
+  return gated_backward_workspace_bytes(m, f, k);
 }
 
 int beam_gated_gemmrc_backward(const void* dC, const void* A, const void* B_gate, const void* B_up, const void* gate,
@@ -204,10 +204,12 @@ int beam_gated_gemmrc_backward(const void* dC, const void* A, const void* B_gate
                                static_cast<cudaStream_t>(stream));
 }
 
+size_t beam_gemmrc_backward_workspace_bytes(int m, int n, int k) { return gemmrc_backward_workspace_bytes(m, n, k); }
+
 int beam_gemmrc_backward(const void* dC, const void* A, const void* B, void* dA, void* dB, int m, int n, int k, int flags,
-                         void* stream) {
+                         void* workspace, size_t workspace_bytes, void* stream) {
   if (flags & ~BEAM_FLAG_BF16) return BEAM_ERR_INVALID_ARG;
-  return launch_gemmrc_backward(dC, A, B, dA, dB, m, n, k, flags & BEAM_FLAG_BF16 ? 1 : 0,
+  return launch_gemmrc_backward(dC, A, B, dA, dB, m, n, k, flags & BEAM_FLAG_BF16 ? 1 : 0, workspace, workspace_bytes,
                                 static_cast<cudaStream_t>(stream));
 }
 

@@ -151,16 +151,38 @@ int launch_gated(const void* A, const void* Bg, const void* Bu, void* C, void* G
 
 namespace {
 
-// Fills in one job of a gradient launch and appends its tiles to the list.
+// One product of a gradient launch (see GradJob).
 struct JobSpec {
   const void* a[2];
   const void* b[2];
   void* c;
   int rows, cols, contraction, segments;
   bool a_mn;
+  int slices = 1;
+
+  long long tiles() const { return static_cast<long long>(ceil_div(rows, 256)) * ceil_div(cols, 256); }
+  int k_blocks() const { return ceil_div(contraction, GradShape::kBK) * segments; }
+  size_t plane_bytes() const { return 4ull * rows * cols; }
+  size_t scratch_bytes() const { return slices > 1 ? (slices * plane_bytes() + 255) / 256 * 256 : 0; }
 };
 
-int add_job(GradParams* p, const JobSpec& s) {
+// How many slices each job's contraction is cut into.  All k-blocks of the launch over all pairs is the time it cannot go below; a
+// job whose tiles take twice that or more (and 8 k-blocks, 2 us) is cut into slices of about that time, at most kMaxSlices.
+// Planned as if all gradients were wanted, so that the bits of one do not depend on which others are asked for.
+// (dA, dBg, dBu) of 333 x 2744 x 1000: 8 tiles of 86 k-blocks and 88 of 6 are 16 k-blocks per pair, so dA is cut in 5.
+constexpr int kMaxSlices = 16;
+void plan_slices(JobSpec* jobs, int n, int pairs) {
+  long long work = 0;
+  for (int i = 0; i < n; ++i) work += jobs[i].tiles() * jobs[i].k_blocks();
+  const long long even = (work + pairs - 1) / pairs;
+  const int share = even < 8 ? 8 : even > (1 << 28) ? (1 << 28) : static_cast<int>(even);
+  for (int i = 0; i < n; ++i) {
+    const int want = jobs[i].k_blocks() / share;
+    jobs[i].slices = want < 2 ? 1 : want > kMaxSlices ? kMaxSlices : want;
+  }
+}
+
+int add_job(GradParams* p, const JobSpec& s, void* scratch) {
   GradJob& job = p->job[p->jobs];
   for (int i = 0; i < s.segments; ++i) {
     int st = s.a_mn ? encode_tmap_2d(&job.tm_a[i], s.a[i], 2, s.contraction, s.rows, s.rows, 64, 64, true)
@@ -168,31 +190,74 @@ int add_job(GradParams* p, const JobSpec& s) {
     if (st == BEAM_OK) st = encode_tmap_2d(&job.tm_b[i], s.b[i], 2, s.contraction, s.cols, s.cols, 64, 64, true);
     if (st != BEAM_OK) return st;
   }
-  const int st = encode_tmap_2d(&job.tm_c, s.c, 2, s.rows, s.cols, s.cols, 32, 64, true);
+  const int st = s.slices > 1 ? encode_tmap_3d_f32(&job.tm_c, scratch, s.slices, s.rows, s.cols, 32, 32)
+                              : encode_tmap_2d(&job.tm_c, s.c, 2, s.rows, s.cols, s.cols, 32, 64, true);
   if (st != BEAM_OK) return st;
   job.rows = s.rows;
   job.cols = s.cols;
   job.contraction = s.contraction;
   job.segments = s.segments;
   job.a_mn = s.a_mn ? 1 : 0;
+  job.slices = s.slices;
   job.m_tiles = ceil_div(s.rows, 256);
   job.n_tiles = ceil_div(s.cols, 256);
-  job.first_tile = p->tiles;
-  p->tiles += job.m_tiles * job.n_tiles;
+  job.first_item = p->items;
+  p->items += job.m_tiles * job.n_tiles * s.slices;
   ++p->jobs;
   return BEAM_OK;
 }
 
-int launch_grad(DeviceCtx* ctx, GradParams* p, cudaStream_t stream) {
+int grad_pairs(DeviceCtx* ctx, int* pairs) {
   static ResidentTable table;
-  int fit = 0;
-  const int st = resident_grid(&table, grad_umma_kernel, ctx, GradShape::kThreads, GradShape::kSmemBytes, 2, &fit);
-  if (st != BEAM_OK) return st;
-  p->group_m = 8;
-  p->status = ctx->status_word;
-  const int clusters = p->tiles < fit ? p->tiles : fit;
-  return launch_dependent(grad_umma_kernel, clusters * 2, GradShape::kThreads, GradShape::kSmemBytes, 2, stream,
-                          "cudaLaunchKernelEx(grad_umma)", *p);
+  return resident_grid(&table, grad_umma_kernel, ctx, GradShape::kThreads, GradShape::kSmemBytes, 2, pairs);
+}
+
+// The pairs that scratch sizes are computed for: the current device's, or 74 without one.
+int planned_pairs() {
+  int st = BEAM_OK, pairs = 0;
+  DeviceCtx* ctx = current_device_ctx(&st);
+  return ctx && grad_pairs(ctx, &pairs) == BEAM_OK ? pairs : 74;
+}
+
+size_t grad_scratch_bytes(const JobSpec* jobs, int n) {
+  size_t bytes = 0;
+  for (int i = 0; i < n; ++i) bytes += jobs[i].scratch_bytes();
+  return bytes;
+}
+
+// Launches the planned jobs that have an output; `scratch` holds grad_scratch_bytes() of them.
+int launch_grad(DeviceCtx* ctx, JobSpec* jobs, int n, int pairs, uint8_t* scratch, int bf16, cudaStream_t stream) {
+  for (int i = 1; i < n; ++i)  // longest items first
+    for (int j = i; j > 0 && jobs[j].k_blocks() / jobs[j].slices > jobs[j - 1].k_blocks() / jobs[j - 1].slices; --j) {
+      const JobSpec t = jobs[j];
+      jobs[j] = jobs[j - 1];
+      jobs[j - 1] = t;
+    }
+  GradParams p = {};
+  GradReduceParams r = {};
+  p.bf16 = r.bf16 = bf16;
+  long long groups = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!jobs[i].c) continue;
+    const int st = add_job(&p, jobs[i], scratch);
+    if (st != BEAM_OK) return st;
+    if (jobs[i].slices > 1) {
+      r.planes[r.jobs] = reinterpret_cast<const float4*>(scratch);
+      r.out[r.jobs] = static_cast<uint4*>(jobs[i].c);
+      r.groups[r.jobs] = static_cast<long long>(jobs[i].rows) * (jobs[i].cols / 8);
+      r.slices[r.jobs] = jobs[i].slices;
+      groups += r.groups[r.jobs++];
+      scratch += jobs[i].scratch_bytes();
+    }
+  }
+  p.group_m = 8;
+  p.status = ctx->status_word;
+  const int clusters = p.items < pairs ? p.items : pairs;
+  const int st = launch_dependent(grad_umma_kernel, clusters * 2, GradShape::kThreads, GradShape::kSmemBytes, 2, stream,
+                                  "cudaLaunchKernelEx(grad_umma)", p);
+  if (st != BEAM_OK || r.jobs == 0) return st;
+  return launch_dependent(grad_reduce_kernel, static_cast<int>((groups + 255) / 256), 256, 0, 1, stream,
+                          "cudaLaunchKernelEx(grad_reduce)", r);
 }
 
 size_t slope_bytes(int m, int f) { return (2ull * m * f + 255) / 256 * 256; }
@@ -215,7 +280,39 @@ int launch_slope(DeviceCtx* ctx, const GatedSlopeParams& p, cudaStream_t stream)
 
 }  // namespace
 
-size_t gated_backward_workspace_bytes(int m, int f) { return m > 0 && f > 0 ? 2 * slope_bytes(m, f) : 0; }
+namespace {
+
+// The products of a gated backward pass and of an rc GEMM's, planned; an output that is not wanted is null.
+void gated_jobs(JobSpec (&jobs)[3], const void* dG, const void* dU, const void* A, const void* Bg, const void* Bu, void* dA,
+                void* dBg, void* dBu, int m, int f, int k, int pairs) {
+  jobs[0] = {{dG, dU}, {Bg, Bu}, dA, m, k, f, 2, false};
+  jobs[1] = {{dG, nullptr}, {A, nullptr}, dBg, f, k, m, 1, true};
+  jobs[2] = {{dU, nullptr}, {A, nullptr}, dBu, f, k, m, 1, true};
+  plan_slices(jobs, 3, pairs);
+}
+
+void rc_jobs(JobSpec (&jobs)[2], const void* dC, const void* A, const void* B, void* dA, void* dB, int m, int n, int k,
+             int pairs) {
+  jobs[0] = {{dC, nullptr}, {B, nullptr}, dA, m, k, n, 1, false};
+  jobs[1] = {{dC, nullptr}, {A, nullptr}, dB, n, k, m, 1, true};
+  plan_slices(jobs, 2, pairs);
+}
+
+}  // namespace
+
+size_t gated_backward_workspace_bytes(int m, int f, int k) {
+  if (check_sizes(m, f, k) != BEAM_OK || check_sizes(f, k, f) != BEAM_OK) return 0;
+  JobSpec jobs[3];
+  gated_jobs(jobs, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, m, f, k, planned_pairs());
+  return 2 * slope_bytes(m, f) + grad_scratch_bytes(jobs, 3);
+}
+
+size_t gemmrc_backward_workspace_bytes(int m, int n, int k) {
+  if (check_sizes(m, n, k) != BEAM_OK || check_sizes(n, k, n) != BEAM_OK) return 0;
+  JobSpec jobs[2];
+  rc_jobs(jobs, nullptr, nullptr, nullptr, nullptr, nullptr, m, n, k, planned_pairs());
+  return grad_scratch_bytes(jobs, 2);
+}
 
 int launch_gated_backward(const void* dC, const void* A, const void* Bg, const void* Bu, const void* G, const void* U,
                           void* dA, void* dBg, void* dBu, int m, int f, int k, int activation, int bf16,
@@ -230,17 +327,23 @@ int launch_gated_backward(const void* dC, const void* A, const void* Bg, const v
   const void* all[] = {dC, A, Bg, Bu, G, U, dA, dBg, dBu, workspace};
   for (const void* q : all)
     if (!aligned16(q)) return BEAM_ERR_ALIGNMENT;
-  if (!workspace || workspace_bytes < gated_backward_workspace_bytes(m, f)) return BEAM_ERR_WORKSPACE;
   const size_t mk = 2ull * m * k, fk = 2ull * f * k, mf = 2ull * m * f;
-  const size_t bytes[] = {mf, mk, fk, fk, mf, mf, mk, fk, fk, gated_backward_workspace_bytes(m, f)};
+  const size_t bytes[] = {mf, mk, fk, fk, mf, mf, mk, fk, fk, workspace_bytes};
   for (int o = 6; o < 10; ++o)
     for (int i = 0; i < o; ++i)
       if (overlap(all[o], bytes[o], all[i], bytes[i])) return BEAM_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < 2 * slope_bytes(m, f)) return BEAM_ERR_WORKSPACE;
   DeviceCtx* ctx = current_device_ctx(&st);
   if (!ctx) return st;
+  int pairs = 0;
+  st = grad_pairs(ctx, &pairs);
+  if (st != BEAM_OK) return st;
 
   uint8_t* dG = static_cast<uint8_t*>(workspace);
   uint8_t* dU = dG + slope_bytes(m, f);
+  JobSpec jobs[3];
+  gated_jobs(jobs, dG, dU, A, Bg, Bu, dA, dBg, dBu, m, f, k, pairs);
+  if (workspace_bytes < 2 * slope_bytes(m, f) + grad_scratch_bytes(jobs, 3)) return BEAM_ERR_WORKSPACE;
   GatedSlopeParams sp = {};
   sp.dc = static_cast<const uint4*>(dC);
   sp.gate = static_cast<const uint4*>(G);
@@ -249,44 +352,35 @@ int launch_gated_backward(const void* dC, const void* A, const void* Bg, const v
   sp.dup = reinterpret_cast<uint4*>(dU);
   sp.count8 = static_cast<long long>(m) * (f / 8);
   sp.act = activation;
-
-  GradParams p = {};
-  p.bf16 = bf16;
-  if (dA) st = add_job(&p, {{dG, dU}, {Bg, Bu}, dA, m, k, f, 2, false});
-  if (st == BEAM_OK && dBg) st = add_job(&p, {{dG, nullptr}, {A, nullptr}, dBg, f, k, m, 1, true});
-  if (st == BEAM_OK && dBu) st = add_job(&p, {{dU, nullptr}, {A, nullptr}, dBu, f, k, m, 1, true});
-  if (st != BEAM_OK) return st;
   st = bf16 ? launch_slope<true>(ctx, sp, stream) : launch_slope<false>(ctx, sp, stream);
   if (st != BEAM_OK) return st;
-  return launch_grad(ctx, &p, stream);
+  return launch_grad(ctx, jobs, 3, pairs, dU + slope_bytes(m, f), bf16, stream);
 }
 
 int launch_gemmrc_backward(const void* dC, const void* A, const void* B, void* dA, void* dB, int m, int n, int k,
-                           int bf16, cudaStream_t stream) {
+                           int bf16, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (!dC || (!dA && !dB) || (dA && !B) || (dB && !A)) return BEAM_ERR_INVALID_ARG;
   int st = check_sizes(m, n, k);
   if (st == BEAM_OK) st = check_sizes(n, k, n);
   if (st != BEAM_OK) return st;
-  const void* all[] = {dC, A, B, dA, dB};
+  const void* all[] = {dC, A, B, dA, dB, workspace};
   for (const void* q : all)
     if (!aligned16(q)) return BEAM_ERR_ALIGNMENT;
   const size_t mk = 2ull * m * k, nk = 2ull * n * k, mn = 2ull * m * n;
-  const size_t bytes[] = {mn, mk, nk, mk, nk};
-  for (int o = 3; o < 5; ++o)
+  const size_t bytes[] = {mn, mk, nk, mk, nk, workspace_bytes};
+  for (int o = 3; o < 6; ++o)
     for (int i = 0; i < o; ++i)
       if (overlap(all[o], bytes[o], all[i], bytes[i])) return BEAM_ERR_INVALID_ARG;
   DeviceCtx* ctx = current_device_ctx(&st);
   if (!ctx) return st;
-  GradParams p = {};
-  p.bf16 = bf16;
-  const JobSpec da = {{dC, nullptr}, {B, nullptr}, dA, m, k, n, 1, false};
-  const JobSpec db = {{dC, nullptr}, {A, nullptr}, dB, n, k, m, 1, true};
-  const bool da_first = n >= m;  // the longer contraction first
-  if (dA && da_first) st = add_job(&p, da);
-  if (st == BEAM_OK && dB) st = add_job(&p, db);
-  if (st == BEAM_OK && dA && !da_first) st = add_job(&p, da);
+  int pairs = 0;
+  st = grad_pairs(ctx, &pairs);
   if (st != BEAM_OK) return st;
-  return launch_grad(ctx, &p, stream);
+  JobSpec jobs[2];
+  rc_jobs(jobs, dC, A, B, dA, dB, m, n, k, pairs);
+  const size_t need = grad_scratch_bytes(jobs, 2);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return BEAM_ERR_WORKSPACE;
+  return launch_grad(ctx, jobs, 2, pairs, static_cast<uint8_t*>(workspace), bf16, stream);
 }
 
 }  // namespace beam

@@ -12,6 +12,10 @@
 // dC's rows are still in L2 when the other product reads them.  Jobs are listed longest contraction first.  A job may
 // have two segments, accumulated one after the other into the same tile: dA = dG Bg + dU Bu needs no second pass.
 //
+// A job with few tiles and a long contraction (dA of a short batch: M rows, but F or N steps) is cut into slices of its
+// contraction, so that it does not keep a few pairs busy while the others are done.  A slice stores its fp32 sums as a plane of
+// scratch and grad_reduce_kernel adds the planes in order (the rule stands beside plan_slices() in feedforward_launch.cu).
+//
 // Tiles are 256 x 256 on a cta_group::2 pair, two TMEM accumulators, fp32 throughout, rounded once at the store.
 // Roles: warp 0 loads the left operand, warp 6 the right one (an N-major k-block is two boxes; one thread issuing all
 // four copies of a k-block would be slower than the tensor pipe), warp 1 issues UMMAs, warps 2..5 are the epilogue.
@@ -26,19 +30,21 @@ constexpr int kMaxGradJobs = 3;
 struct GradJob {
   CUtensorMap tm_a[2];  // left operand of each segment: [rows, contraction], box 128 x 64, or M-major: box 64 x 64
   CUtensorMap tm_b[2];  // right operand of each segment: [contraction, columns], box 64 x 64
-  CUtensorMap tm_c;     // [rows, columns], store box 32 rows x 64 columns
+  CUtensorMap tm_c;     // [rows, columns], store box 32 rows x 64 columns; of a sliced job the scratch planes
+                        // [slices][rows][columns] fp32, store box 32 rows x 32 columns
   int rows, cols;
   int contraction;      // of each segment
   int segments;
   int a_mn;             // the left operand is M-major
+  int slices;           // of the contraction over all segments
   int m_tiles, n_tiles;
-  int first_tile;       // of this job in the launch's list
+  int first_item;       // of this job in the launch's list: an item is a tile, or a slice of one
 };
 
 struct GradParams {
   GradJob job[kMaxGradJobs];
   int jobs;
-  int tiles;
+  int items;
   int group_m;
   int bf16;
   int* status;
@@ -58,18 +64,28 @@ struct GradShape {
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
 };
 
-__device__ __forceinline__ const GradJob& grad_tile(const GradParams& p, int t, int& mt, int& nt) {
+struct GradItem {
+  int mt, nt;
+  int kb0, kb1;  // k-blocks, counted over all segments
+  int slice;
+};
+__device__ __forceinline__ const GradJob& grad_item(const GradParams& p, int t, GradItem& w) {
   int i = 0;
-  while (i + 1 < p.jobs && t >= p.job[i + 1].first_tile) ++i;
+  while (i + 1 < p.jobs && t >= p.job[i + 1].first_item) ++i;
   const GradJob& job = p.job[i];
-  t -= job.first_tile;
+  t -= job.first_item;
+  w.slice = t % job.slices;
+  t /= job.slices;
   const int per_group = p.group_m * job.n_tiles;
   const int g = t / per_group;
   const int first_m = g * p.group_m;
   const int rows = min(p.group_m, job.m_tiles - first_m);
   const int r = t - g * per_group;
-  mt = first_m + r % rows;
-  nt = r / rows;
+  w.mt = first_m + r % rows;
+  w.nt = r / rows;
+  const int all = (job.contraction + GradShape::kBK - 1) / GradShape::kBK * job.segments;
+  w.kb0 = all * w.slice / job.slices;
+  w.kb1 = all * (w.slice + 1) / job.slices;
   return job;
 }
 
@@ -124,39 +140,39 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
     const bool left = warp == 0;
     uint32_t s = 0, ph = 0;
     bool alive = true;
-    for (int t = first; alive && t < p.tiles; t += stride) {
-      int mt, nt;
-      const GradJob& job = grad_tile(p, t, mt, nt);
-      const int row = mt * 256 + cta_rank * 128;
-      const int col = nt * 256 + cta_rank * 128;
+    for (int t = first; alive && t < p.items; t += stride) {
+      GradItem w;
+      const GradJob& job = grad_item(p, t, w);
+      const int row = w.mt * 256 + cta_rank * 128;
+      const int col = w.nt * 256 + cta_rank * 128;
       const int num_kb = (job.contraction + S::kBK - 1) / S::kBK;
-      for (int seg = 0; alive && seg < job.segments; ++seg) {
+      for (int at = w.kb0; at < w.kb1; ++at) {
+        const int seg = at >= num_kb ? 1 : 0;
+        const int kb = at - seg * num_kb;
         const CUtensorMap* map = left ? &job.tm_a[seg] : &job.tm_b[seg];
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) {
-            alive = false;
-            break;
+        if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) {
+          alive = false;
+          break;
+        }
+        if (ptx::elect_one()) {
+          // The left producer of the leader arms the barrier with all bytes of both CTAs; bytes of the right operand that
+          // land before that only make the pending count negative for a moment, the phase still needs the arrive.
+          if (left && leader) ptx::mbar_arrive_expect_tx(full_bar(s), 2u * S::kStageBytes);
+          const uint32_t bar = ptx::mapa(full_bar(s), 0);
+          const uint32_t a = smem_base + s * S::kStageBytes;
+          if (left && !job.a_mn) {
+            ptx::tma_load_2d_pair(a, map, bar, kb * S::kBK, row);
+          } else {
+            const uint32_t dst = left ? a : a + S::kABytes;
+            const int along = left ? row : col;
+            ptx::tma_load_2d_pair(dst, map, bar, along, kb * S::kBK);
+            ptx::tma_load_2d_pair(dst + 8192u, map, bar, along + 64, kb * S::kBK);
           }
-          if (ptx::elect_one()) {
-            // The left producer of the leader arms the barrier with all bytes of both CTAs; bytes of the right operand
-            // that land before that only make the pending count negative for a moment, the phase still needs the arrive.
-            if (left && leader) ptx::mbar_arrive_expect_tx(full_bar(s), 2u * S::kStageBytes);
-            const uint32_t bar = ptx::mapa(full_bar(s), 0);
-            const uint32_t a = smem_base + s * S::kStageBytes;
-            if (left && !job.a_mn) {
-              ptx::tma_load_2d_pair(a, map, bar, kb * S::kBK, row);
-            } else {
-              const uint32_t dst = left ? a : a + S::kABytes;
-              const int along = left ? row : col;
-              ptx::tma_load_2d_pair(dst, map, bar, along, kb * S::kBK);
-              ptx::tma_load_2d_pair(dst + 8192u, map, bar, along + 64, kb * S::kBK);
-            }
-          }
-          __syncwarp();
-          if (++s == S::kStages) {
-            s = 0;
-            ph ^= 1u;
-          }
+        }
+        __syncwarp();
+        if (++s == S::kStages) {
+          s = 0;
+          ph ^= 1u;
         }
       }
     }
@@ -171,9 +187,9 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
       constexpr uint64_t kDescStride = S::kStageBytes >> 4;
       uint32_t s = 0, ph = 0;
       bool alive = true;
-      for (int t = first, j = 0; alive && t < p.tiles; t += stride, ++j) {
-        int mt, nt;
-        const GradJob& job = grad_tile(p, t, mt, nt);
+      for (int t = first, j = 0; alive && t < p.items; t += stride, ++j) {
+        GradItem w;
+        const GradJob& job = grad_item(p, t, w);
         const uint32_t acc = static_cast<uint32_t>(j) & 1u;
         const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
         if (!bounded_wait_converged(tmem_empty_bar(acc), acc_ph ^ 1u, cta_abort, p.status, kFaultMmaWaitAcc, lane)) break;
@@ -182,8 +198,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
         const uint32_t idesc = idesc0 | (job.a_mn ? ptx::kIdescAMnMajor : 0u);
         const uint64_t a_desc0 = job.a_mn ? a_desc_mn : a_desc_k;
         const uint64_t a_step = job.a_mn ? (2048 >> 4) : (32 >> 4);  // 16 steps of the contraction
-        const int num_kb = (job.contraction + S::kBK - 1) / S::kBK * job.segments;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!bounded_wait_converged(full_bar(s), ph, cta_abort, p.status, kFaultMmaWaitFull, lane)) {
             alive = false;
             break;
@@ -193,7 +208,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
             const uint64_t a = a_desc0 + s * kDescStride, b = b_desc0 + s * kDescStride;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
-              ptx::umma_f16<2>(d_tmem, a + i * a_step, b + i * (2048 >> 4), idesc, (kb > 0 || i > 0) ? 1u : 0u);
+              ptx::umma_f16<2>(d_tmem, a + i * a_step, b + i * (2048 >> 4), idesc, (kb > w.kb0 || i > 0) ? 1u : 0u);
             ptx::umma_commit_pair_both(empty_bar(s), 0x3);
           }
           __syncwarp();
@@ -211,27 +226,35 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
     const uint32_t quad = warp & 3u;
     const uint32_t lead_empty0 = ptx::mapa(tmem_empty_bar(0), 0);
     uint32_t stores = 0;
-    for (int t = first, j = 0; t < p.tiles; t += stride, ++j) {
-      int mt, nt;
-      const GradJob& job = grad_tile(p, t, mt, nt);
+    for (int t = first, j = 0; t < p.items; t += stride, ++j) {
+      GradItem w;
+      const GradJob& job = grad_item(p, t, w);
       const uint32_t acc = static_cast<uint32_t>(j) & 1u;
       const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
       if (!bounded_wait_warp(tmem_full_bar(acc), acc_ph, cta_abort, p.status, kFaultEpilogueWait, lane)) break;
       ptx::tc_fence_after();
-      const int row0 = mt * 256 + cta_rank * 128 + static_cast<int>(quad) * 32;
+      const int row0 = w.mt * 256 + cta_rank * 128 + static_cast<int>(quad) * 32;
       const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * 256u;
+      const bool sliced = job.slices > 1;
+      const int step = sliced ? 32 : 64;  // columns in 128 bytes
 #pragma unroll 1
-      for (int c = 0; c < 256; c += 64) {
-        const int col = nt * 256 + c;
+      for (int c = 0; c < 256; c += step) {
+        const int col = w.nt * 256 + c;
         if (row0 >= job.rows || col >= job.cols) break;  // warp-uniform
-        uint32_t v0[32], v1[32], out[32];
-        ptx::tmem_ld_32x32(taddr + c, v0);
-        ptx::tmem_ld_32x32(taddr + c + 32, v1);
-        ptx::tmem_ld_wait();
+        uint32_t out[32];
+        ptx::tmem_ld_32x32(taddr + c, out);
+        if (!sliced) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32(taddr + c + 32, v);
+          ptx::tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          out[q] = ptx::pack_out2(__uint_as_float(v0[2 * q]), __uint_as_float(v0[2 * q + 1]), p.bf16);
-          out[16 + q] = ptx::pack_out2(__uint_as_float(v1[2 * q]), __uint_as_float(v1[2 * q + 1]), p.bf16);
+          for (int q = 0; q < 16; ++q)
+            out[q] = ptx::pack_out2(__uint_as_float(out[2 * q]), __uint_as_float(out[2 * q + 1]), p.bf16);
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            out[16 + q] = ptx::pack_out2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]), p.bf16);
+        } else {
+          ptx::tmem_ld_wait();
         }
         const uint32_t buf = staging_base + (quad * 2u + (stores & 1u)) * S::kBufBytes;
         if (stores >= 2) {
@@ -245,7 +268,10 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          ptx::tma_store_2d(&job.tm_c, buf, col, row0);
+          if (sliced)
+            ptx::tma_store_3d(&job.tm_c, buf, col, row0, w.slice);
+          else
+            ptx::tma_store_2d(&job.tm_c, buf, col, row0);
           ptx::tma_store_commit();
         }
         ++stores;
@@ -256,7 +282,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
     }
   }
 
-  if (warp >= 2 && warp < 6 && lane == 0) ptx::tma_store_wait_read<0>();
+  if (warp >= 2 && warp < 6 && lane == 0) ptx::tma_store_wait_all<0>();
   __syncwarp();
   if (*cta_abort) abort_drain_delay();
   ptx::tc_fence_before();
@@ -266,6 +292,36 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
     ptx::tc_fence_after();
     ptx::tmem_dealloc<2>(tmem_base, 512);
   }
+}
+
+// Adds the planes of the sliced jobs, in the order of the slices, and rounds once.  A thread does 8 columns.
+struct GradReduceParams {
+  const float4* planes[kMaxGradJobs];
+  uint4* out[kMaxGradJobs];
+  long long groups[kMaxGradJobs];  // of 8 elements
+  int slices[kMaxGradJobs];
+  int jobs;
+  int bf16;
+};
+
+static __global__ void __launch_bounds__(256) grad_reduce_kernel(const GradReduceParams p) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  int i = 0;
+  while (i < p.jobs && at >= p.groups[i]) at -= p.groups[i++];
+  if (i == p.jobs) return;
+  const long long plane = 2 * p.groups[i];
+  const float4* from = p.planes[i] + 2 * at;
+  float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+#pragma unroll 4
+  for (int s = 0; s < p.slices[i]; ++s) {
+    const float4 a = __ldcs(from + s * plane), b = __ldcs(from + s * plane + 1);
+    lo.x += a.x; lo.y += a.y; lo.z += a.z; lo.w += a.w;
+    hi.x += b.x; hi.y += b.y; hi.z += b.z; hi.w += b.w;
+  }
+  p.out[i][at] = make_uint4(ptx::pack_out2(lo.x, lo.y, p.bf16), ptx::pack_out2(lo.z, lo.w, p.bf16),
+                            ptx::pack_out2(hi.x, hi.y, p.bf16), ptx::pack_out2(hi.z, hi.w, p.bf16));
 }
 
 }  // namespace beam

@@ -84,7 +84,7 @@ int launch_instance(DeviceCtx* ctx, const NarrowPlan& plan, int resident, const 
   if (st == BEAM_OK) st = encode_tmap_2d_u8(&p.tm_b, B, n, k / 2, static_cast<uint32_t>(p.width / kCta), 128);
   if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sa, sa, ceil_div(m, 128), words, 1, 128);
   if (st == BEAM_OK) st = encode_tmap_2d_words64(&p.tm_sb, sb, ceil_div(n, 128), words, S::kScaleBlocksB, 128);
-  if (st == BEAM_OK && kCta == 2) st = encode_tmap_2d(&p.tm_c, C, 2, m, n, n, 32, 64, true);
+  if (st == BEAM_OK && kCta == 2) st = encode_tmap_2d_sw64(&p.tm_c, C, m, n, n, 32, 32);
   if (st != BEAM_OK) return st;
   const int ctas = kCta * p.split;
   return launch_dependent(mxfp4_umma_kernel<kCta>, clusters * ctas, S::kThreads, p.bar_offset + S::kBarBytes, ctas, stream,

@@ -166,13 +166,13 @@ static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint
 //              rows of A are loaded, two issuers take turns at the stages, and clusters may share a contraction, all
 //              as in gated_umma.cuh.
 //
-// Roles: warp 0 loads A and its scales, warp 6 B and its scales, warps 1 and 7 issue, warps 2..5 are the epilogue.
+// Roles: warp 0 loads A and its scales, warp 10 B and its scales, warps 1 and 11 issue, warps 2..9 are the epilogue.
 struct MxGemmParams {
   CUtensorMap tm_a;   // packed A [M, K / 2 bytes], box (rows per CTA) x 128
   CUtensorMap tm_b;   // packed B [N, K / 2 bytes], box (width / kCta) x 128
   CUtensorMap tm_sa;  // scales of A as 8-byte words [row blocks][64 ceil(K / 128)], box 1 x 128
   CUtensorMap tm_sb;  // scales of B, box 2 x 128
-  CUtensorMap tm_c;   // pair: C [M, N], store box 32 rows x 64 columns
+  CUtensorMap tm_c;   // pair: C [M, N], store box 32 rows x 32 columns, 64 B swizzle
   void* c;
   int m, n, k;
   int width;          // columns per tile
@@ -194,14 +194,17 @@ struct MxShape {
   static constexpr int kScaleBlocksB = kCta;  // row blocks of B's scales per tile
   static constexpr int kScaleBytes = (1 + kScaleBlocksB) * 1024;
   static constexpr int kMaxStages = 16;
-  static constexpr int kThreads = 256;  // warp 7: the second issuer
+  // warps: 0 and 10 producers, 1 and 11 issuers, 2..9 epilogue (two for each quarter of the lanes, taking turns at the columns)
+  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kSecondProducer = 2 + kEpilogueWarps;
+  static constexpr int kSecondIssuer = kSecondProducer + 1;
+  static constexpr int kThreads = 32 * (kSecondIssuer + 1);
   static constexpr int kMaxWidth = kCta == 2 ? 256 : 128;
   static constexpr int kAccStep = kCta == 2 ? 192 : 128;  // TMEM columns from one accumulator to the other
   static constexpr int kScaleCols = kAccStep + kMaxWidth;  // first column of the scales
   static constexpr int kScaleHalf = 4 + 4 * kScaleBlocksB;  // columns of 128 elements of K
   static constexpr int kScaleSet = 2 * kScaleHalf;          // ... of a stage; an issuer alternates between two sets
-  static constexpr int kBufsPerWarp = 1;
-  static constexpr int kStagingBytes = kCta == 2 ? 4 * kBufsPerWarp * 4096 : 0;
+  static constexpr int kStagingBytes = kCta == 2 ? kEpilogueWarps * 2048 : 0;  // a box of 32 rows x 32 columns per warp
   static constexpr int kBarBytes = 512;
   static constexpr int kSmemLimit = 232448;
   static constexpr int kRingBytes = kSmemLimit - kStagingBytes - kBarBytes;
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
     }
     for (uint32_t a = 0; a < 2; ++a) {
       ptx::mbar_init(tmem_full_bar(a), static_cast<uint32_t>(p.issuers));
-      ptx::mbar_init(tmem_empty_bar(a), 4 * kCta);
+      ptx::mbar_init(tmem_empty_bar(a), S::kEpilogueWarps * kCta);
     }
     *cta_abort = 0;
     ptx::fence_mbar_init();
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0 || warp == 6) {
+  if (warp == 0 || warp == S::kSecondProducer) {
     // ------------------------------------------------------------------ TMA producers
     ptx::grid_dependency_wait();  // before the first global read
     const bool left = warp == 0;
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
         }
       }
     }
-  } else if (warp == 1 || warp == 7) {
+  } else if (warp == 1 || warp == S::kSecondIssuer) {
     // ------------------------------------------------------------------ MMA issuers (two: see gated_umma.cuh)
     const uint32_t issuers = static_cast<uint32_t>(p.issuers);
     const uint32_t mine = warp == 1 ? 0u : 1u;
@@ -440,10 +443,11 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
       }
     }
   } else if (kCta == 2 || p.split == 1) {
-    // ------------------------------------------------------------------ epilogue (warps 2..5)
+    // ------------------------------------------------------------------ epilogue (warps 2..9)
     const uint32_t quad = warp & 3u;
+    const int half = static_cast<int>(warp - 2u) >> 2;
     const uint32_t lead_empty0 = (kCta == 2) ? ptx::mapa(tmem_empty_bar(0), 0) : tmem_empty_bar(0);
-    uint32_t stores = 0;
+    bool stored = false;  // this warp's staging buffer has been handed to a bulk store
     for (int t = first, j = 0; t < tiles; t += stride, ++j) {
       const uint32_t acc = static_cast<uint32_t>(j) & 1u;
       const uint32_t acc_ph = (static_cast<uint32_t>(j) >> 1) & 1u;
@@ -455,47 +459,53 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
       const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * S::kAccStep;
       if constexpr (kCta == 2) {
         // Columns in chunks of 64, the chunk that the other accumulator shares first: the last of an even tile, the first
-        // of an odd one.
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int c = 64 * (acc == 0 ? (i + 3) & 3 : i);
-          const int col = nt * 256 + c;
-          uint32_t v0[32], v1[32], out[32];
-          ptx::tmem_ld_32x32(taddr + c, v0);
-          ptx::tmem_ld_32x32(taddr + c + 32, v1);
-          ptx::tmem_ld_wait();
-          if (i == 0) {
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cluster(lead_empty0);
-          }
-          if (row0 >= p.m || col >= p.n) continue;  // warp-uniform
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            out[q] = ptx::pack_out2(__uint_as_float(v0[2 * q]), __uint_as_float(v0[2 * q + 1]), p.bf16);
-            out[16 + q] = ptx::pack_out2(__uint_as_float(v1[2 * q]), __uint_as_float(v1[2 * q + 1]), p.bf16);
-          }
-          const uint32_t buf = staging_base + (quad * S::kBufsPerWarp + stores % S::kBufsPerWarp) * 4096u;
-          if (stores >= S::kBufsPerWarp) {
-            if (lane == 0) ptx::tma_store_wait_read<S::kBufsPerWarp - 1>();
-            __syncwarp();
-          }
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            ptx::st_shared_v4(buf + lane * 128u + ((static_cast<uint32_t>(q) ^ (lane & 7u)) << 4), out[4 * q],
-                              out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]);
-          ptx::fence_proxy_async_smem();
+        // of an odd one.  The two warps of a quarter take turns, so the first of them reads that chunk; the other's arrive
+        // says that it has done with the tile before, whose accumulator the next tile goes into.
+        const uint32_t buf = staging_base + (warp - 2u) * 2048u;
+        auto hand_back = [&]() {
+          ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            ptx::tma_store_2d(&p.tm_c, buf, col, row0);
-            ptx::tma_store_commit();
+          if (lane == 0) ptx::mbar_arrive_cluster(lead_empty0);
+        };
+        if (half == 1) hand_back();
+#pragma unroll 1
+        for (int i = half; i < 4; i += 2) {
+          const int c = 64 * (acc == 0 ? (i + 3) & 3 : i);
+          uint32_t v[2][32];
+          ptx::tmem_ld_32x32(taddr + c, v[0]);
+          ptx::tmem_ld_32x32(taddr + c + 32, v[1]);
+          ptx::tmem_ld_wait();
+          if (i == 0) hand_back();
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const int col = nt * 256 + c + 32 * part;
+            if (row0 >= p.m || col >= p.n) continue;  // warp-uniform
+            uint32_t out[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+              out[q] = ptx::pack_out2(__uint_as_float(v[part][2 * q]), __uint_as_float(v[part][2 * q + 1]), p.bf16);
+            if (stored) {
+              if (lane == 0) ptx::tma_store_wait_read<0>();
+              __syncwarp();
+            }
+            // the 64-byte swizzle (see gated_umma.cuh)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              ptx::st_shared_v4(buf + lane * 64u + ((static_cast<uint32_t>(q) ^ ((lane >> 1) & 3u)) << 4), out[4 * q],
+                                out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              ptx::tma_store_2d(&p.tm_c, buf, col, row0);
+              ptx::tma_store_commit();
+            }
+            stored = true;
           }
-          ++stores;
         }
       } else {
         const int col0 = nt * p.width;
         const int row = row0 + static_cast<int>(lane);
-        for (int c = 0; row0 < p.m && c < p.width && col0 + c < p.n; c += 32) {
+        for (int c = 32 * half; row0 < p.m && c < p.width && col0 + c < p.n; c += 64) {
           uint32_t v[32];
           mx_load(p, taddr + c, v);
           mx_store_row(p, v, row, col0 + c, 32);
@@ -511,23 +521,27 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
     if (p.split > 1) {
       // ---------------------------------------------------------------- a tile shared by a cluster: its epilogue
       const uint32_t split = static_cast<uint32_t>(p.split);
+      const bool epilogue = warp >= 2 && warp < 2 + S::kEpilogueWarps;
       const uint32_t quad = warp & 3u;
+      const int half = epilogue ? static_cast<int>(warp - 2u) >> 2 : 0;
       const uint32_t row = quad * 32u + lane;
       const uint32_t taddr = tmem_base + ((quad * 32u) << 16);
       const int slice = p.width / p.split;  // columns that each CTA finishes, a multiple of 8
       const uint32_t groups = static_cast<uint32_t>(slice) / 4u;
       bool ready = false;
-      if (warp >= 2 && warp < 6) {
+      if (epilogue) {
         ready = bounded_wait_warp(tmem_full_bar(0), 0, cta_abort, p.status, kFaultEpilogueWait, lane);
         ptx::tc_fence_after();
         ready = ready && static_cast<int>(quad * 32u) < p.m;
       }
       ptx::cluster_sync_all();  // every CTA's operands have been multiplied: the rings may be written over
       if (ready) {
+        int turn = 0;
         for (uint32_t to = 0; to < split; ++to) {
           if (to == k_rank) continue;
           const uint32_t there = ptx::mapa(smem_base, to);
           for (int c = 0; c < slice; c += 32) {
+            if ((turn++ & 1) != half) continue;
             uint32_t v[32];
             mx_load(p, taddr + to * slice + c, v);
             if (static_cast<int>(row) < p.m)
@@ -538,7 +552,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
       ptx::cluster_sync_all();
       if (ready) {
         const int col0 = first * p.width + static_cast<int>(k_rank) * slice;
-        for (int c = 0; c < slice && col0 + c < p.n; c += 32) {
+        for (int c = 32 * half; c < slice && col0 + c < p.n; c += 64) {
           uint32_t v[32];
           mx_load(p, taddr + k_rank * slice + c, v);
           exchange_sum(smem_base, k_rank, split, groups, static_cast<uint32_t>(c) / 4u, row, v, slice - c);
@@ -548,7 +562,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
     }
   }
 
-  if (kCta == 2 && warp >= 2 && warp < 6 && lane == 0) ptx::tma_store_wait_read<0>();
+  if (kCta == 2 && warp >= 2 && warp < 2 + S::kEpilogueWarps && lane == 0) ptx::tma_store_wait_read<0>();
   __syncwarp();
   if (*cta_abort) abort_drain_delay();
   ptx::tc_fence_before();

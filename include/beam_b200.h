@@ -246,7 +246,8 @@ BEAM_API int beam_gemmrc_silu(const void* A, const void* B, void* C, int m, int 
 BEAM_API int beam_gated_gemmrc(const void* A, const void* B_gate, const void* B_up, void* C, void* gate, void* up, int m,
                                int f, int k, int activation, int flags, void* stream);
 
-/* Scratch bytes for beam_gated_gemmrc_backward: dG and dU. */
+/* Scratch bytes for beam_gated_gemmrc_backward on the current device: dG and dU, and for problems with few tiles and long
+ * contractions the fp32 sums of slices of those. */
 BEAM_API size_t beam_gated_gemmrc_backward_workspace_bytes(int m, int f, int k);
 
 /* Gradients of beam_gated_gemmrc, given dC [M,F] and the kept gate and up:
@@ -260,9 +261,13 @@ BEAM_API int beam_gated_gemmrc_backward(const void* dC, const void* A, const voi
                                         size_t workspace_bytes, void* stream);
 
 /* Gradients of the rc GEMM C = A x B^T: dA[M,K] = dC[M,N] x B[N,K] and dB[N,K] = dC^T x A[M,K], in one launch, without
- * transposing anything in memory.  fp16, or bf16 with BEAM_FLAG_BF16.  dA or dB may be NULL (then B, or A, may be too). */
+ * transposing anything in memory.  fp16, or bf16 with BEAM_FLAG_BF16.  dA or dB may be NULL (then B, or A, may be too).
+ * Where there are few tiles, a long contraction is cut into slices whose fp32 sums go through `workspace` and are added in a fixed
+ * order by a second launch; beam_gemmrc_backward_workspace_bytes says how much that takes on the current device (0 for
+ * most sizes; workspace may then be NULL). */
+BEAM_API size_t beam_gemmrc_backward_workspace_bytes(int m, int n, int k);
 BEAM_API int beam_gemmrc_backward(const void* dC, const void* A, const void* B, void* dA, void* dB, int m, int n, int k,
-                                  int flags, void* stream);
+                                  int flags, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- MXFP4: microscaled 4-bit floating point ------------------------------------------------------- */
 

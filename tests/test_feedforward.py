@@ -157,6 +157,8 @@ def test_c_entries_refuse_bad_arguments(built_library):
     need = L.beam_gated_gemmrc_backward_workspace_bytes
     need.restype, need.argtypes = sz, [i, i, i]
     assert need(64, 64, 64) == 2 * 64 * 64 * 2 and need(3, 8, 64) == 2 * 256 and need(0, 8, 8) == 0
+    # 74 pairs without a device: dA of 16 rows is 4 tiles of 512 k-blocks, the weights' 512 tiles of one: 34 k-blocks per pair
+    assert need(16, 16384, 1024) == 2 * 16 * 16384 * 2 + 512 // 35 * 16 * 1024 * 4
     f = L.beam_gated_gemmrc_backward
     f.argtypes = [vp] * 9 + [i, i, i, i, i, vp, sz, vp]
     good = p[:9] + [64, 64, 64, 1, 2, p[9], need(64, 64, 64), None]
@@ -170,15 +172,21 @@ def test_c_entries_refuse_bad_arguments(built_library):
     assert call(f, good, _6=p[1]) == 1 and call(f, good, _7=p[8]) == 1 and call(f, good, _14=p[4]) == 1
     assert call(f, good, _8=p[8] + 8) == 3
 
+    need = L.beam_gemmrc_backward_workspace_bytes
+    need.restype, need.argtypes = sz, [i, i, i]
+    assert need(64, 64, 64) == 0 and need(8192, 4096, 8192) == 0 and need(64, 60, 64) == 0
+    # dA is one tile of 64 k-blocks, in slices of 8; dB 16 tiles of one k-block
+    assert need(64, 4096, 256) == 8 * 64 * 256 * 4
     f = L.beam_gemmrc_backward
-    f.argtypes = [vp] * 5 + [i, i, i, i, vp]
-    good = p[:5] + [64, 64, 64, 0, None]
+    f.argtypes = [vp] * 5 + [i, i, i, i, vp, sz, vp]
+    good = p[:5] + [64, 64, 64, 0, None, 0, None]
     assert call(f, good) == 8
     assert call(f, good, _3=None, _2=None) == 8 and call(f, good, _4=None, _1=None) == 8
     assert call(f, good, _3=None, _4=None) == 1 and call(f, good, _0=None) == 1
     assert call(f, good, _1=None) == 1 and call(f, good, _2=None) == 1
     assert call(f, good, _6=12) == 3 and call(f, good, _5=0) == 1 and call(f, good, _8=16) == 1
     assert call(f, good, _3=p[4]) == 1 and call(f, good, _4=p[0]) == 1
+    assert call(f, good, _9=p[3], _10=64) == 1 and call(f, good, _9=p[9] + 4, _10=64) == 3
 
 
 def test_python_refuses_cpu_tensors_and_bad_names(beam):
@@ -292,7 +300,7 @@ def test_gated_passes_nan_and_infinity_on(beam, healthy):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("m,f,k", [(1, 8, 8), (3, 72, 264), (64, 64, 64), (130, 520, 200), (257, 264, 1032),
-                                   (1000, 776, 328)])
+                                   (1000, 776, 328), (17, 4104, 136), (300, 2744, 264), (2500, 64, 264)])
 def test_gated_backward(beam, healthy, dtype, act, m, f, k):
     a, bg, bu = gated_inputs(m, f, k, dtype, m + f)
     gate, up, dc = normal((m, f), dtype, 5, 2.0), normal((m, f), dtype, 6), normal((m, f), dtype, 7)
@@ -321,7 +329,7 @@ def test_gated_backward_of_each_gradient_alone(beam, healthy):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 8, 8), (5, 64, 72), (127, 136, 200), (256, 256, 256), (300, 1000, 1096),
-                                   (1000, 264, 520), (2000, 48, 24)])
+                                   (1000, 264, 520), (2000, 48, 24), (40, 4104, 264), (3000, 264, 136)])
 def test_gemmrc_backward(beam, healthy, dtype, m, n, k):
     dc, a, b = normal((m, n), dtype, 1), normal((m, k), dtype, 2), normal((n, k), dtype, 3)
     room = [torch.full((r + 2, k), 3.0, dtype=dtype, device="cuda") for r in (m, n)]
