@@ -201,8 +201,8 @@ int add_job(GradParams* p, const JobSpec& s, void* scratch) {
   job.slices = s.slices;
   job.m_tiles = ceil_div(s.rows, 256);
   job.n_tiles = ceil_div(s.cols, 256);
-  job.first_item = p->items;
-  p->items += job.m_tiles * job.n_tiles * s.slices;
+  job.first_item = p->end;
+  p->end += job.m_tiles * job.n_tiles * s.slices;
   ++p->jobs;
   return BEAM_OK;
 }
@@ -252,9 +252,23 @@ int launch_grad(DeviceCtx* ctx, JobSpec* jobs, int n, int pairs, uint8_t* scratc
   }
   p.group_m = 8;
   p.status = ctx->status_word;
-  const int clusters = p.items < pairs ? p.items : pairs;
-  const int st = launch_dependent(grad_umma_kernel, clusters * 2, GradShape::kThreads, GradShape::kSmemBytes, 2, stream,
-                                  "cudaLaunchKernelEx(grad_umma)", p);
+  // Launches of whole waves, each at least kLaunchKBlocks k-blocks per pair (see grad_umma.cuh); a small list is one launch.
+  constexpr int kLaunchKBlocks = 1024;  // 0.28 ms
+  const int items = p.end;
+  int st = BEAM_OK;
+  for (p.begin = 0; p.begin < items && st == BEAM_OK; p.begin = p.end) {
+    long long k_blocks = 0;
+    int end = p.begin;
+    for (int j = 0; end < items && k_blocks < kLaunchKBlocks; end += pairs) {
+      while (j + 1 < p.jobs && end >= p.job[j + 1].first_item) ++j;
+      k_blocks += ceil_div(p.job[j].contraction, GradShape::kBK) * p.job[j].segments / p.job[j].slices;
+      if (k_blocks == 0) k_blocks = 1;
+    }
+    p.end = end < items ? end : items;
+    const int clusters = p.end - p.begin < pairs ? p.end - p.begin : pairs;
+    st = launch_dependent(grad_umma_kernel, clusters * 2, GradShape::kThreads, GradShape::kSmemBytes, 2, stream,
+                          "cudaLaunchKernelEx(grad_umma)", p);
+  }
   if (st != BEAM_OK || r.jobs == 0) return st;
   return launch_dependent(grad_reduce_kernel, static_cast<int>((groups + 255) / 256), 256, 0, 1, stream,
                           "cudaLaunchKernelEx(grad_reduce)", r);

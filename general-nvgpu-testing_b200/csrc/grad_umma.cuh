@@ -12,6 +12,11 @@
 // dC's rows are still in L2 when the other product reads them.  Jobs are listed longest contraction first.  A job may
 // have two segments, accumulated one after the other into the same tile: dA = dG Bg + dU Bu needs no second pass.
 //
+// A long list is cut into launches of whole waves.  Pairs drift apart over many tiles, and what they no longer read at the same
+// time comes from memory again: all gradients of 8192 x 16384 x 4096 read 10.8 GB in one launch against 7.8 GB in two (dA; dBg
+// and dBu), and memory traffic costs clock under the power cap.  Sustained, with all waves in one launch / 14 / 7 / 4 / 2 / 1
+// waves per launch: 3806 / 3564 / 3525 / 3516 / 3534 / 3612 us.
+//
 // A job with few tiles and a long contraction (dA of a short batch: M rows, but F or N steps) is cut into slices of its
 // contraction, so that it does not keep a few pairs busy while the others are done.  A slice stores its fp32 sums as a plane of
 // scratch and grad_reduce_kernel adds the planes in order (the rule stands beside plan_slices() in feedforward_launch.cu).
@@ -44,7 +49,7 @@ struct GradJob {
 struct GradParams {
   GradJob job[kMaxGradJobs];
   int jobs;
-  int items;
+  int begin, end;  // this launch's part of the list of items
   int group_m;
   int bf16;
   int* status;
@@ -96,7 +101,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
   const uint32_t lane = threadIdx.x & 31;
   const int cta_rank = static_cast<int>(ptx::cluster_ctarank());
   const bool leader = cta_rank == 0;
-  const int first = static_cast<int>(blockIdx.x >> 1);
+  const int first = p.begin + static_cast<int>(blockIdx.x >> 1);
   const int stride = static_cast<int>(gridDim.x >> 1);
 
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -140,7 +145,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
     const bool left = warp == 0;
     uint32_t s = 0, ph = 0;
     bool alive = true;
-    for (int t = first; alive && t < p.items; t += stride) {
+    for (int t = first; alive && t < p.end; t += stride) {
       GradItem w;
       const GradJob& job = grad_item(p, t, w);
       const int row = w.mt * 256 + cta_rank * 128;
@@ -187,7 +192,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
       constexpr uint64_t kDescStride = S::kStageBytes >> 4;
       uint32_t s = 0, ph = 0;
       bool alive = true;
-      for (int t = first, j = 0; alive && t < p.items; t += stride, ++j) {
+      for (int t = first, j = 0; alive && t < p.end; t += stride, ++j) {
         GradItem w;
         const GradJob& job = grad_item(p, t, w);
         const uint32_t acc = static_cast<uint32_t>(j) & 1u;
@@ -226,7 +231,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
     const uint32_t quad = warp & 3u;
     const uint32_t lead_empty0 = ptx::mapa(tmem_empty_bar(0), 0);
     uint32_t stores = 0;
-    for (int t = first, j = 0; t < p.items; t += stride, ++j) {
+    for (int t = first, j = 0; t < p.end; t += stride, ++j) {
       GradItem w;
       const GradJob& job = grad_item(p, t, w);
       const uint32_t acc = static_cast<uint32_t>(j) & 1u;
