@@ -59,7 +59,7 @@ struct MxQuantParams {
 };
 
 template <bool kBf16>
-static __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxQuantParams p) {
+static __global__ void __launch_bounds__(256, 8) mxfp4_quantize_kernel(const MxQuantParams p) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   const MxPlace at = mx_place(p.units);
