@@ -18,7 +18,7 @@ const char* beam_status_string(int status) {
     case BEAM_OK: return "ok";
     case BEAM_ERR_INVALID_ARG: return "invalid argument (null pointer, non-positive size or bad value)";
     case BEAM_ERR_UNSUPPORTED: return "unsupported shape, tile or split factor";
-    case BEAM_ERR_ALIGNMENT: return "alignment: pointers must be 16-byte aligned, K and N multiples of 8";
+    case BEAM_ERR_ALIGNMENT: return "alignment: pointers must be 16-byte aligned, K and N multiples of 8 (MXFP4: K of 32)";
     case BEAM_ERR_WORKSPACE: return "workspace missing or too small";
     case BEAM_ERR_CUDA: return "CUDA runtime call failed";
     case BEAM_ERR_TENSORMAP: return "TMA descriptor rejected by the driver";

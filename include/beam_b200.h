@@ -37,7 +37,7 @@ extern "C" {
 #define BEAM_OK 0
 #define BEAM_ERR_INVALID_ARG 1     /* null pointer, non-positive size, bad enum */
 #define BEAM_ERR_UNSUPPORTED 2     /* shape / tile / split factor this build cannot run */
-#define BEAM_ERR_ALIGNMENT 3       /* pointer not 16-byte aligned or K, N not multiples of 8 */
+#define BEAM_ERR_ALIGNMENT 3       /* pointer not 16-byte aligned or K, N not multiples of 8 (MXFP4: K of 32) */
 #define BEAM_ERR_WORKSPACE 4       /* workspace missing or too small */
 #define BEAM_ERR_CUDA 5            /* a CUDA runtime call failed (see beam_last_cuda_error) */
 #define BEAM_ERR_TENSORMAP 6       /* the driver refused a TMA descriptor */
@@ -251,7 +251,8 @@ BEAM_API int beam_gated_gemmrc(const void* A, const void* B_gate, const void* B_
 BEAM_API size_t beam_gated_gemmrc_backward_workspace_bytes(int m, int f, int k);
 
 /* Gradients of beam_gated_gemmrc, given dC [M,F] and the kept gate and up:
- *   dG = dC * up * act'(gate), dU = dC * act(gate)      (fp32, rounded once to the operands' type, in `workspace`)
+ *   dG = dC * up * act'(gate), dU = dC * act(gate)      (fp32, rounded once to the operands' type, in `workspace`: in fp16
+ *                                                        they overflow above 65504, like any operand)
  *   dA = dG x B_gate + dU x B_up,  dB_gate = dG^T x A,  dB_up = dU^T x A      (fp32 accumulation, one rounding)
  * Any of dA, dB_gate and dB_up may be NULL, but not all three; B_gate and B_up may be NULL without dA, and A without dB_gate and
  * dB_up.  Outputs are overwritten (no accumulation into them), and overlap neither the inputs nor each other nor the workspace. */

@@ -474,3 +474,102 @@ def test_refusals_on_the_device(beam):
         beam.gemmrc_backward(c, a, bg)
     with pytest.raises(ValueError):
         beam.gemmrc_backward(c, a, bg, da=a)                         # in place
+
+
+@pytest.mark.gpu
+def test_two_graphs_replayed_at_once(beam, healthy):
+    """Graphs captured one after the other on one stream own their scratch: replayed on two streams at the same time they give what
+    they give alone."""
+    made = []
+    for j in range(2):
+        a, bg, bu = gated_inputs(333, 1096, 520, torch.bfloat16, 70 + j)
+        rest = [normal((333, 1096), torch.bfloat16, 80 + 3 * j + i) for i in range(3)]
+        args = [rest[0], a, bg, bu, rest[1], rest[2]]
+        outs = [torch.empty_like(t) for t in (a, bg, bu)]
+        beam.gated_gemmrc_backward(*args, *outs)
+        made.append((args, outs, [t.clone() for t in outs]))
+    torch.cuda.synchronize()
+    stream, graphs = torch.cuda.Stream(), []
+    for args, outs, _ in made:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            beam.gated_gemmrc_backward(*args, *outs)
+        graphs.append(graph)
+    for _, outs, _ in made:
+        for t in outs:
+            t.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, outs, want in made:
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", (5, 300))
+def test_views_inside_larger_tensors(beam, healthy, m):
+    """Contiguous views that start 16 bytes into an allocation are taken as they are; a start that is no multiple of 16 bytes is
+    refused."""
+    f, k = 264, 200
+
+    def inside(t, offset):
+        room = torch.full((t.numel() + 64,), 5.0, dtype=t.dtype, device="cuda")
+        view = room[offset:offset + t.numel()].view(t.shape)
+        view.copy_(t)
+        return room, view
+
+    a, bg, bu = gated_inputs(m, f, k, torch.float16, 11)
+    rooms = [inside(t, 8) for t in (a, bg, bu, torch.zeros(m, f, dtype=torch.float16, device="cuda"))]
+    (_, va), (_, vg), (_, vu), (room, c) = rooms
+    beam.gated_gemmrc(va, vg, vu, c)
+    check_gated(a, bg, bu, "silu", c)
+    assert (room[:8] == 5).all() and (room[8 + c.numel():] == 5).all()
+    for j in range(4):
+        args = [va, vg, vu, c]
+        args[j] = inside(args[j], 4)[1]
+        with pytest.raises(ValueError, match="alignment"):
+            beam.gated_gemmrc(*args)
+
+
+@pytest.mark.gpu
+def test_offsets_past_two_to_the_31(beam, healthy):
+    """More than 2^31 output elements: the last rows are right."""
+    m, f, k = 135000, 16384, 64
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    a, bg, bu = gated_inputs(m, f, k, torch.bfloat16, 13)
+    c = torch.empty(m, f, dtype=torch.bfloat16, device="cuda")
+    beam.gated_gemmrc(a, bg, bu, c, activation="relu")
+    check_gated(a[-300:], bg, bu, "relu", c[-300:])
+    check_gated(a[:300], bg, bu, "relu", c[:300])
+    da = torch.empty_like(a)
+    beam.gemmrc_backward(c, a, bg, da=da)
+    left, right = c[-300:].double(), bg.double().t()
+    want = left @ right.t()
+    check(da[-300:], want, half_step(c.dtype) * want.abs() + 1.01 * summing(left, right))
+
+
+@pytest.mark.gpu
+def test_same_bits_every_time(beam, healthy):
+    """Shared contractions, slices and two issuers add in a fixed order: equal bits from run to run, also while the device is busy."""
+    noise = normal((4096, 4096), torch.bfloat16, 1)
+    for m, f, k in ((3, 1000, 4104), (100, 2000, 2056), (300, 2744, 520)):
+        a, bg, bu = gated_inputs(m, f, k, torch.bfloat16, 90)
+        gate, up, dc = (normal((m, f), torch.bfloat16, 91 + j) for j in range(3))
+        seen = []
+        for j in range(4):
+            c = torch.empty(m, f, dtype=torch.bfloat16, device="cuda")
+            grads = [torch.empty_like(t) for t in (a, bg, bu)]
+            if j:
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    torch.matmul(noise, noise)
+            beam.gated_gemmrc(a, bg, bu, c)
+            beam.gated_gemmrc_backward(dc, a, bg, bu, gate, up, *grads)
+            seen.append([c] + grads)
+        torch.cuda.synchronize()
+        for other in seen[1:]:
+            assert all(torch.equal(x, y) for x, y in zip(seen[0], other)), (m, f, k)

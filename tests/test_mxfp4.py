@@ -305,3 +305,37 @@ def test_refusals_on_the_device(beam):
         beam.mxfp4_gemmrc(q, s, q[:, :16].contiguous(), s, c)
     with pytest.raises(ValueError):
         beam.mxfp4_gemmrc(q, s, q[:12].contiguous(), s, c[:, :12].contiguous())  # N no multiple of 8
+
+
+@pytest.mark.gpu
+def test_offsets_past_two_to_the_31(beam, healthy):
+    """More than 2^31 elements to 4 bits and back, and a product whose second operand starts past 2^31: the last rows are right."""
+    rows, k = 70000, 32768
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    q, s = beam.mxfp4_empty(rows, k)
+    beam.mxfp4_quantize(x, q, s)
+    y = torch.empty_like(x)
+    beam.mxfp4_dequantize(q, s, y)
+    for part in (slice(0, 200), slice(rows - 200, rows)):
+        assert torch.equal(y[part], round64(x[part])[0].bfloat16())
+    del y
+    a = matrix(4, k, torch.bfloat16, 2)
+    c = torch.empty(4, rows, dtype=torch.bfloat16, device="cuda")
+    beam.mxfp4_gemmrc(*quantized(beam, a), q, s, c)
+    check_product(c[:, -200:].contiguous(), round64(a)[0], round64(x[-200:])[0])
+
+
+@pytest.mark.gpu
+def test_bad_placement_is_refused(beam):
+    x = matrix(4, 64, torch.float16, 1)
+    q, s = quantized(beam, x)
+    room = torch.zeros(4 * 32 + 8, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="alignment"):
+        beam.mxfp4_quantize(x, room[8:136].view(4, 32), s)
+    with pytest.raises(ValueError):  # scales inside q's memory
+        big = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+        beam.mxfp4_quantize(x, big[:128].view(4, 32), big[64:576].view(1, 1, 512))
+    with pytest.raises(ValueError):  # a view with gaps
+        beam.mxfp4_quantize(x[::2], q[:2], s)
