@@ -70,18 +70,24 @@ struct GatedShape {
   static_assert((2 * kMaxStages + 4) * 8 + 8 <= kBarBytes, "barrier block too small");
 };
 
+// g = act(g) * u in the first `columns` of 32 columns, a multiple of 8 (warp-uniform: a narrow tile has few).
 template <int kAct>
-__device__ __forceinline__ void gated_combine(uint32_t (&g)[32], const uint32_t (&u)[32]) {
+__device__ __forceinline__ void gated_combine(uint32_t (&g)[32], const uint32_t (&u)[32], int columns) {
 #pragma unroll
-  for (int q = 0; q < 32; ++q)
-    g[q] = __float_as_uint(act_value<kAct>(__uint_as_float(g[q])) * __uint_as_float(u[q]));
+  for (int i = 0; i < 32; i += 8) {
+    if (i < columns) {
+#pragma unroll
+      for (int q = i; q < i + 8; ++q)
+        g[q] = __float_as_uint(act_value<kAct>(__uint_as_float(g[q])) * __uint_as_float(u[q]));
+    }
+  }
 }
-__device__ __forceinline__ void gated_combine(int act, uint32_t (&g)[32], const uint32_t (&u)[32]) {
+__device__ __forceinline__ void gated_combine(int act, uint32_t (&g)[32], const uint32_t (&u)[32], int columns) {
   switch (act) {  // warp-uniform
-    case kActSilu: gated_combine<kActSilu>(g, u); break;
-    case kActGelu: gated_combine<kActGelu>(g, u); break;
-    case kActGeluTanh: gated_combine<kActGeluTanh>(g, u); break;
-    default: gated_combine<kActRelu>(g, u); break;
+    case kActSilu: gated_combine<kActSilu>(g, u, columns); break;
+    case kActGelu: gated_combine<kActGelu>(g, u, columns); break;
+    case kActGeluTanh: gated_combine<kActGeluTanh>(g, u, columns); break;
+    default: gated_combine<kActRelu>(g, u, columns); break;
   }
 }
 
@@ -155,21 +161,56 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
     nt = r / rows;
   };
 
-  if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < static_cast<uint32_t>(p.stages); ++s) {
-      ptx::mbar_init(full_bar(s), 1);
-      ptx::mbar_init(empty_bar(s), 1);
+  const uint32_t b_bytes = static_cast<uint32_t>(p.width) * 128u;
+  const uint32_t stage_tx = 2u * b_bytes + static_cast<uint32_t>(kCta) * static_cast<uint32_t>(p.a_bytes);
+  // One CTA: the loads of k-block kb into stage s (the ring of a pair: see the producers).
+  auto load_stage = [&](uint32_t s, int kb, int row_a, int row_b) {
+    const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
+    const uint32_t b = a + static_cast<uint32_t>(p.a_bytes);
+    const int k0 = (kb_base + kb) * S::kBK;
+    ptx::mbar_arrive_expect_tx(full_bar(s), stage_tx);
+    ptx::tma_load_2d(b, &p.tm_gate, full_bar(s), k0, row_b);
+    ptx::tma_load_2d(b + b_bytes, &p.tm_up, full_bar(s), k0, row_b);
+    ptx::tma_load_2d(a, &p.tm_a, full_bar(s), k0, row_a);
+  };
+  // k-blocks whose loads one thread puts in flight before the CTA-wide set-up barrier (two stages at least are there)
+  const int preloaded = kCta == 1 ? min(num_kb, 2) : 0;
+  if (warp == 0) {
+    if (lane < static_cast<uint32_t>(p.stages)) {
+      ptx::mbar_init(full_bar(lane), 1);
+      ptx::mbar_init(empty_bar(lane), 1);
     }
-    for (uint32_t a = 0; a < 2; ++a) {
-      ptx::mbar_init(tmem_full_bar(a), static_cast<uint32_t>(p.issuers));
-      ptx::mbar_init(tmem_empty_bar(a), 4 * kCta);  // one arrive per epilogue warp of each CTA
+    if (lane < 2) {
+      ptx::mbar_init(tmem_full_bar(lane), static_cast<uint32_t>(p.issuers));
+      ptx::mbar_init(tmem_empty_bar(lane), 4 * kCta);  // one arrive per epilogue warp of each CTA
     }
-    *cta_abort = 0;
     ptx::fence_mbar_init();
-    ptx::prefetch_tensormap(&p.tm_a);
-    ptx::prefetch_tensormap(&p.tm_gate);
-    ptx::prefetch_tensormap(&p.tm_up);
-    ptx::grid_launch_dependents();  // the next kernel on the stream may set itself up; it waits for this grid itself
+    __syncwarp();
+    if (lane == 0) {
+      *cta_abort = 0;
+      ptx::prefetch_tensormap(&p.tm_a);
+      ptx::prefetch_tensormap(&p.tm_gate);
+      ptx::prefetch_tensormap(&p.tm_up);
+      ptx::grid_launch_dependents();  // the next kernel on the stream may set itself up; it waits for this grid itself
+    }
+    __syncwarp();
+    if constexpr (kCta == 1) {
+      // The weights' first k-blocks may come into L2 while the kernel before this one finishes: a prefetch reads nothing, so
+      // it does not matter whether that kernel still writes them.  16 x 8192 x 4096: 25.7 -> 24.9 us; not worth its
+      // issue for narrow tiles (4 x 1024 x 2048: 7.3 -> 7.5).
+      if (p.width > 32 && ptx::elect_one()) {
+        for (int kb = 0; kb < min(num_kb, p.stages); ++kb) {  // one row of tiles: tile = column tile
+          ptx::tma_prefetch_2d(&p.tm_gate, (kb_base + kb) * S::kBK, first * p.width);
+          ptx::tma_prefetch_2d(&p.tm_up, (kb_base + kb) * S::kBK, first * p.width);
+        }
+      }
+      __syncwarp();
+      ptx::grid_dependency_wait();  // before the first global read
+      if (ptx::elect_one()) {
+        for (int kb = 0; kb < preloaded; ++kb) load_stage(static_cast<uint32_t>(kb), kb, 0, first * p.width);
+      }
+      __syncwarp();
+    }
   }
   if (warp == 1) {
     ptx::tmem_alloc<kCta>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -183,25 +224,12 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
 
   if (warp == 0 || (warp >= 6 && warp < S::kSecondIssuer)) {
     // ------------------------------------------------------------------ TMA producers
-    if constexpr (kCta == 1) {
-      // The weights' first k-blocks may come into L2 while the kernel before this one finishes: a prefetch reads nothing, so
-      // it does not matter whether that kernel still writes them.  16 x 8192 x 4096: 25.7 -> 24.9 us; not worth its
-      // issue for narrow tiles (4 x 1024 x 2048: 7.3 -> 7.5).
-      if (p.width > 32 && ptx::elect_one()) {
-        const CUtensorMap* map = warp == 0 ? &p.tm_gate : &p.tm_up;
-        for (int kb = 0; kb < min(num_kb, p.stages); ++kb)
-          ptx::tma_prefetch_2d(map, (kb_base + kb) * S::kBK, first * p.width);  // one row of tiles: tile = column tile
-      }
-      __syncwarp();
-    }
     ptx::grid_dependency_wait();  // before the first global read; everything else follows from these reads
-    const uint32_t b_bytes = static_cast<uint32_t>(p.width) * 128u;
-    const uint32_t bytes = 2u * b_bytes + static_cast<uint32_t>(kCta) * static_cast<uint32_t>(p.a_rows) * 128u;
     const uint32_t mine = warp == 0 ? 0u : warp - 5u;  // this warp fills every kProducers-th stage of the walk
     const uint32_t stages = static_cast<uint32_t>(p.stages);
     const CUtensorMap* tm_b = leader ? &p.tm_gate : &p.tm_up;
-    uint32_t s = mine % stages, ph = (mine / stages) & 1u;
-    int kb = static_cast<int>(mine);
+    int kb = static_cast<int>(mine) + (preloaded + 1 - static_cast<int>(mine)) / 2 * 2;  // its first that is not in flight yet
+    uint32_t s = static_cast<uint32_t>(kb) % stages, ph = (static_cast<uint32_t>(kb) / stages) & 1u;
     for (int t = first; t < tiles; t += stride) {
       int mt, nt;
       tile_at(t, mt, nt);
@@ -210,18 +238,14 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
       for (; kb < num_kb; kb += S::kProducers) {
         if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) break;
         if (ptx::elect_one()) {
-          const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
-          const uint32_t b = a + static_cast<uint32_t>(p.a_bytes);
-          if (leader) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
-          const int k0 = (kb_base + kb) * S::kBK;
           if constexpr (kCta == 2) {
+            const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
+            if (leader) ptx::mbar_arrive_expect_tx(full_bar(s), stage_tx);
             const uint32_t bar = ptx::mapa(full_bar(s), 0);
-            ptx::tma_load_2d_pair(a, &p.tm_a, bar, k0, row_a);
-            ptx::tma_load_2d_pair(b, tm_b, bar, k0, row_b);
+            ptx::tma_load_2d_pair(a, &p.tm_a, bar, kb * S::kBK, row_a);
+            ptx::tma_load_2d_pair(a + static_cast<uint32_t>(p.a_bytes), tm_b, bar, kb * S::kBK, row_b);
           } else {
-            ptx::tma_load_2d(b, &p.tm_gate, full_bar(s), k0, row_b);
-            ptx::tma_load_2d(b + b_bytes, &p.tm_up, full_bar(s), k0, row_b);
-            ptx::tma_load_2d(a, &p.tm_a, full_bar(s), k0, row_a);
+            load_stage(s, kb, row_a, row_b);
           }
         }
         __syncwarp();
@@ -342,7 +366,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
           store(g, 1);
           store(u, 2);
         }
-        gated_combine(p.act, g, u);
+        gated_combine(p.act, g, u, kCta == 2 ? 32 : p.width - c);
         store(g, 0);
       }
       ptx::tc_fence_before();
@@ -408,7 +432,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
             store(g, 1);
             store(u, 2);
           }
-          gated_combine(p.act, g, u);
+          gated_combine(p.act, g, u, slice - c);
           store(g, 0);
         }
       }
