@@ -116,18 +116,21 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
       smem_gen + S::kStages * S::kStageBytes + S::kStagingBytes + 8 * (2 * S::kStages + 4));
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < S::kStages; ++s) {
-      ptx::mbar_init(full_bar(s), 1);
-      ptx::mbar_init(empty_bar(s), 1);
+  if (warp == 0) {
+    if (lane < S::kStages) {
+      ptx::mbar_init(full_bar(lane), 1);
+      ptx::mbar_init(empty_bar(lane), 1);
     }
-    for (uint32_t a = 0; a < 2; ++a) {
-      ptx::mbar_init(tmem_full_bar(a), 1);
-      ptx::mbar_init(tmem_empty_bar(a), 8);  // one arrive per epilogue warp of each CTA
+    if (lane < 2) {
+      ptx::mbar_init(tmem_full_bar(lane), 1);
+      ptx::mbar_init(tmem_empty_bar(lane), 8);  // one arrive per epilogue warp of each CTA
     }
-    *cta_abort = 0;
     ptx::fence_mbar_init();
-    ptx::grid_launch_dependents();
+    if (lane == 0) {
+      *cta_abort = 0;
+      ptx::grid_launch_dependents();
+    }
+    __syncwarp();
   }
   if (warp == 1) {
     ptx::tmem_alloc<2>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);

@@ -282,22 +282,73 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
     nt = r / rows;
   };
 
-  if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < static_cast<uint32_t>(p.stages); ++s) {
-      ptx::mbar_init(full_bar(s), 1);
-      ptx::mbar_init(empty_bar(s), 1);
+  const uint32_t stage_tx = static_cast<uint32_t>(kCta) * (a_bytes + b_bytes + static_cast<uint32_t>(S::kScaleBytes));
+  // k-blocks that one thread puts in flight before the CTA-wide set-up barrier (see gated_umma.cuh)
+  const int preloaded = kCta == 1 ? min(num_kb, 2) : 0;
+  // The loads of A (left) or B of k-block kb into stage s.  A's thread arms the barrier with the whole stage; B's bytes may land
+  // before that (see grad_umma.cuh).
+  auto load_stage = [&](bool left, uint32_t s, int kb, int block_a, int col) {
+    const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
+    const uint32_t b = a + a_bytes;
+    const uint32_t sf = b + b_bytes;
+    const int x = (kb_base + kb) * 128;
+    if (left && leader) ptx::mbar_arrive_expect_tx(full_bar(s), stage_tx);
+    if constexpr (kCta == 2) {
+      const uint32_t bar = ptx::mapa(full_bar(s), 0);
+      if (left) {
+        ptx::tma_load_2d_pair(a, &p.tm_a, bar, x, block_a * 128);
+        ptx::tma_load_2d_pair(sf, &p.tm_sa, bar, x, block_a);
+      } else {
+        ptx::tma_load_2d_pair(b, &p.tm_b, bar, x, col + cta_rank * 128);
+        ptx::tma_load_2d_pair(sf + 1024u, &p.tm_sb, bar, x, col >> 7);
+      }
+    } else {
+      if (left) {
+        ptx::tma_load_2d(a, &p.tm_a, full_bar(s), x, block_a * 128);
+        ptx::tma_load_2d(sf, &p.tm_sa, full_bar(s), x, block_a);
+      } else {
+        ptx::tma_load_2d(b, &p.tm_b, full_bar(s), x, col);
+        ptx::tma_load_2d(sf + 1024u, &p.tm_sb, full_bar(s), x, col >> 7);
+      }
     }
-    for (uint32_t a = 0; a < 2; ++a) {
-      ptx::mbar_init(tmem_full_bar(a), static_cast<uint32_t>(p.issuers));
-      ptx::mbar_init(tmem_empty_bar(a), S::kEpilogueWarps * kCta);
+  };
+  if (warp == 0) {
+    if (lane < static_cast<uint32_t>(p.stages)) {
+      ptx::mbar_init(full_bar(lane), 1);
+      ptx::mbar_init(empty_bar(lane), 1);
     }
-    *cta_abort = 0;
+    if (lane < 2) {
+      ptx::mbar_init(tmem_full_bar(lane), static_cast<uint32_t>(p.issuers));
+      ptx::mbar_init(tmem_empty_bar(lane), S::kEpilogueWarps * kCta);
+    }
     ptx::fence_mbar_init();
-    ptx::prefetch_tensormap(&p.tm_a);
-    ptx::prefetch_tensormap(&p.tm_b);
-    ptx::prefetch_tensormap(&p.tm_sa);
-    ptx::prefetch_tensormap(&p.tm_sb);
-    ptx::grid_launch_dependents();
+    __syncwarp();
+    if (lane == 0) {
+      *cta_abort = 0;
+      ptx::prefetch_tensormap(&p.tm_a);
+      ptx::prefetch_tensormap(&p.tm_b);
+      ptx::prefetch_tensormap(&p.tm_sa);
+      ptx::prefetch_tensormap(&p.tm_sb);
+      ptx::grid_launch_dependents();
+    }
+    __syncwarp();
+    if constexpr (kCta == 1) {
+      // B's first stages may come into L2 while the kernel before this one finishes (see gated_umma.cuh).  Wide tiles only:
+      // 1 x 16384 x 8192 with its quantisation 17.6 -> 16.9 us, but 16 x 8192 x 8192 (64-wide tiles) 13.0 -> 13.7.
+      if (p.width > 64 && ptx::elect_one()) {
+        for (int kb = 0; kb < min(num_kb, p.stages); ++kb)
+          ptx::tma_prefetch_2d(&p.tm_b, (kb_base + kb) * 128, first * p.width);
+      }
+      __syncwarp();
+      ptx::grid_dependency_wait();  // before the first global read
+      if (ptx::elect_one()) {
+        for (int kb = 0; kb < preloaded; ++kb) {
+          load_stage(true, static_cast<uint32_t>(kb), kb, 0, first * p.width);
+          load_stage(false, static_cast<uint32_t>(kb), kb, 0, first * p.width);
+        }
+      }
+      __syncwarp();
+    }
   }
   if (warp == 1) {
     ptx::tmem_alloc<kCta>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -312,63 +363,27 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
   if (warp == 0 || warp == S::kSecondProducer) {
     // ------------------------------------------------------------------ TMA producers
     const bool left = warp == 0;
-    if constexpr (kCta == 1) {
-      // B's first stages may come into L2 while the kernel before this one finishes (see gated_umma.cuh).  Wide tiles only:
-      // 1 x 16384 x 8192 with its quantisation 17.6 -> 16.9 us, but 16 x 8192 x 8192 (64-wide tiles) 13.0 -> 13.7.
-      if (!left && p.width > 64 && ptx::elect_one()) {
-        for (int kb = 0; kb < min(num_kb, p.stages); ++kb)
-          ptx::tma_prefetch_2d(&p.tm_b, (kb_base + kb) * 128, first * p.width);
-      }
-      __syncwarp();
-    }
     ptx::grid_dependency_wait();  // before the first global read
-    const uint32_t bytes = static_cast<uint32_t>(kCta) *
-                           (static_cast<uint32_t>(p.a_rows) * 128u + b_bytes + static_cast<uint32_t>(S::kScaleBytes));
     const uint32_t stages = static_cast<uint32_t>(p.stages);
-    uint32_t s = 0, ph = 0;
+    int kb = preloaded;  // at most the ring
+    uint32_t s = static_cast<uint32_t>(kb) % stages, ph = static_cast<uint32_t>(kb) / stages;
     bool alive = true;
     for (int t = first; alive && t < tiles; t += stride) {
       int mt, nt;
       tile_at(t, mt, nt);
-      const int block_a = mt * kCta + cta_rank;  // row block of A: 128 rows, one row of scale blocks
-      const int col = nt * p.width;
-      for (int kb = 0; kb < num_kb; ++kb) {
+      for (; kb < num_kb; ++kb) {
         if (!bounded_wait_converged(empty_bar(s), ph ^ 1u, cta_abort, p.status, kFaultProducerWait, lane)) {
           alive = false;
           break;
         }
-        if (ptx::elect_one()) {
-          const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
-          const uint32_t b = a + a_bytes;
-          const uint32_t sf = b + b_bytes;
-          const int x = (kb_base + kb) * 128;
-          // A's producer arms the barrier with the whole stage; B's bytes may land before that (see grad_umma.cuh).
-          if (left && leader) ptx::mbar_arrive_expect_tx(full_bar(s), bytes);
-          if constexpr (kCta == 2) {
-            const uint32_t bar = ptx::mapa(full_bar(s), 0);
-            if (left) {
-              ptx::tma_load_2d_pair(a, &p.tm_a, bar, x, block_a * 128);
-              ptx::tma_load_2d_pair(sf, &p.tm_sa, bar, x, block_a);
-            } else {
-              ptx::tma_load_2d_pair(b, &p.tm_b, bar, x, col + cta_rank * 128);
-              ptx::tma_load_2d_pair(sf + 1024u, &p.tm_sb, bar, x, col >> 7);
-            }
-          } else {
-            if (left) {
-              ptx::tma_load_2d(a, &p.tm_a, full_bar(s), x, block_a * 128);
-              ptx::tma_load_2d(sf, &p.tm_sa, full_bar(s), x, block_a);
-            } else {
-              ptx::tma_load_2d(b, &p.tm_b, full_bar(s), x, col);
-              ptx::tma_load_2d(sf + 1024u, &p.tm_sb, full_bar(s), x, col >> 7);
-            }
-          }
-        }
+        if (ptx::elect_one()) load_stage(left, s, kb, mt * kCta + cta_rank, nt * p.width);
         __syncwarp();
         if (++s == stages) {
           s = 0;
           ph ^= 1u;
         }
       }
+      kb = 0;
     }
   } else if (warp == 1 || warp == S::kSecondIssuer) {
     // ------------------------------------------------------------------ MMA issuers (two: see gated_umma.cuh)
