@@ -377,10 +377,10 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 _HALF_TYPES = (torch.float16, torch.bfloat16)
 
 
-def _check_matrix(name, t, shape, dtype, device):
-    """A contiguous CUDA tensor of this shape, type and device; shape or device None: any of two dimensions, any CUDA device;
+def _check_matrix(name, t, shape, dtype, index):
+    """A contiguous tensor of this shape and type on CUDA device `index`; shape or index None: any of two dimensions, any CUDA device;
     dtype may be a tuple of choices."""
-    if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.device == device
+    if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.get_device() == index
             and t.is_contiguous()):
         return  # the usual case, by few tests: a call's host time is of the order of a small kernel's
     if not isinstance(t, torch.Tensor):
@@ -393,8 +393,8 @@ def _check_matrix(name, t, shape, dtype, device):
         raise ValueError("%s must be contiguous" % name)
     if t.dim() != (2 if shape is None else len(shape)) or (shape is not None and tuple(t.shape) != tuple(shape)):
         raise ValueError("%s must be %s, got %s" % (name, "2-D" if shape is None else tuple(shape), tuple(t.shape)))
-    if device is not None and t.device != device:
-        raise ValueError("%s must be on %s, like the other tensors" % (name, device))
+    if index is not None and t.get_device() != index:
+        raise ValueError("%s must be on cuda:%d, like the other tensors" % (name, index))
 
 
 def _check_first(name, t, dtypes):
@@ -422,30 +422,31 @@ def _half_flags(t):
     return 2 if t.dtype == torch.bfloat16 else 0
 
 
-# The current stream's handle of a device, without building a torch.cuda.Stream (2 us a call) where torch offers that.
+# The current device and the current stream's handle of a device, without building torch.cuda objects (2 us a call) where torch
+# offers that.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(fn_name, device, *args):
-    """Calls a C entry with `device` current, on torch's current stream of that device (its last argument)."""
+def _call(fn_name, index, *args):
+    """Calls a C entry with device `index` current, on torch's current stream of that device (its last argument)."""
     fn = getattr(_lib or _load(), fn_name)
-    index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         st = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             st = fn(*args, _raw_stream(index))
     if st != BEAM_OK:
         _raise(st, fn_name)
 
 
-def _sized(fn_name, device, *sizes):
+def _sized(fn_name, index, *sizes):
     """A workspace size, which goes by the device."""
     fn = getattr(_lib or _load(), fn_name)
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == index:
         return fn(*sizes)
-    with torch.cuda.device(device):
+    with torch.cuda.device(index):
         return fn(*sizes)
 
 
@@ -457,16 +458,16 @@ def gated_gemmrc(a, b_gate, b_up, c, activation="silu", gate=None, up=None):
     gate and up, given together, are [M,F] outputs that keep the two products for gated_gemmrc_backward."""
     act = _activation(activation)
     m, k = _check_first("a", a, _HALF_TYPES)
-    dtype, device, f = a.dtype, a.device, _rows(b_gate)
-    _check_matrix("b_gate", b_gate, (f, k), dtype, device)
-    _check_matrix("b_up", b_up, (f, k), dtype, device)
-    _check_matrix("c", c, (m, f), dtype, device)
+    dtype, dev, f = a.dtype, a.get_device(), _rows(b_gate)
+    _check_matrix("b_gate", b_gate, (f, k), dtype, dev)
+    _check_matrix("b_up", b_up, (f, k), dtype, dev)
+    _check_matrix("c", c, (m, f), dtype, dev)
     if (gate is None) != (up is None):
         raise ValueError("gate and up must be given together")
     if gate is not None:
-        _check_matrix("gate", gate, (m, f), dtype, device)
-        _check_matrix("up", up, (m, f), dtype, device)
-    _call("beam_gated_gemmrc", device, a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(), c.data_ptr(), _ptr(gate),
+        _check_matrix("gate", gate, (m, f), dtype, dev)
+        _check_matrix("up", up, (m, f), dtype, dev)
+    _call("beam_gated_gemmrc", dev, a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(), c.data_ptr(), _ptr(gate),
           _ptr(up), m, f, k, act, _half_flags(a))
 
 
@@ -480,23 +481,23 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
     held in scratch of 4 M F bytes (and more for short batches) from torch's allocator."""
     act = _activation(activation)
     m, k = _check_first("a", a, _HALF_TYPES)
-    dtype, device, f = a.dtype, a.device, _rows(b_gate)
+    dtype, dev, f = a.dtype, a.get_device(), _rows(b_gate)
     if da is None and db_gate is None and db_up is None:
         raise ValueError("at least one of da, db_gate and db_up must be given")
-    _check_matrix("b_gate", b_gate, (f, k), dtype, device)
-    _check_matrix("b_up", b_up, (f, k), dtype, device)
-    _check_matrix("dc", dc, (m, f), dtype, device)
-    _check_matrix("gate", gate, (m, f), dtype, device)
-    _check_matrix("up", up, (m, f), dtype, device)
+    _check_matrix("b_gate", b_gate, (f, k), dtype, dev)
+    _check_matrix("b_up", b_up, (f, k), dtype, dev)
+    _check_matrix("dc", dc, (m, f), dtype, dev)
+    _check_matrix("gate", gate, (m, f), dtype, dev)
+    _check_matrix("up", up, (m, f), dtype, dev)
     if da is not None:
-        _check_matrix("da", da, (m, k), dtype, device)
+        _check_matrix("da", da, (m, k), dtype, dev)
     if db_gate is not None:
-        _check_matrix("db_gate", db_gate, (f, k), dtype, device)
+        _check_matrix("db_gate", db_gate, (f, k), dtype, dev)
     if db_up is not None:
-        _check_matrix("db_up", db_up, (f, k), dtype, device)
-    nbytes = _sized("beam_gated_gemmrc_backward_workspace_bytes", device, m, f, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _call("beam_gated_gemmrc_backward", device, dc.data_ptr(), a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(),
+        _check_matrix("db_up", db_up, (f, k), dtype, dev)
+    nbytes = _sized("beam_gated_gemmrc_backward_workspace_bytes", dev, m, f, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+    _call("beam_gated_gemmrc_backward", dev, dc.data_ptr(), a.data_ptr(), b_gate.data_ptr(), b_up.data_ptr(),
           gate.data_ptr(), up.data_ptr(), _ptr(da), _ptr(db_gate), _ptr(db_up), m, f, k, act, _half_flags(a),
           ws.data_ptr(), nbytes)
 
@@ -505,18 +506,18 @@ def gemmrc_backward(dc, a, b, da=None, db=None):
     """Gradients of c = a @ b.T: da[M,K] = dc[M,N] @ b[N,K] and db[N,K] = dc.T @ a[M,K], in one launch.  All tensors
     float16 or all bfloat16; the gradients wanted are given (at least one) and overwritten; N and K multiples of 8."""
     m, k = _check_first("a", a, _HALF_TYPES)
-    dtype, device, n = a.dtype, a.device, _rows(b)
-    _check_matrix("b", b, (n, k), dtype, device)
-    _check_matrix("dc", dc, (m, n), dtype, device)
+    dtype, dev, n = a.dtype, a.get_device(), _rows(b)
+    _check_matrix("b", b, (n, k), dtype, dev)
+    _check_matrix("dc", dc, (m, n), dtype, dev)
     if da is None and db is None:
         raise ValueError("at least one of da and db must be given")
     if da is not None:
-        _check_matrix("da", da, (m, k), dtype, device)
+        _check_matrix("da", da, (m, k), dtype, dev)
     if db is not None:
-        _check_matrix("db", db, (n, k), dtype, device)
-    nbytes = _sized("beam_gemmrc_backward_workspace_bytes", device, m, n, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _call("beam_gemmrc_backward", device, dc.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(da), _ptr(db), m, n, k,
+        _check_matrix("db", db, (n, k), dtype, dev)
+    nbytes = _sized("beam_gemmrc_backward_workspace_bytes", dev, m, n, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
+    _call("beam_gemmrc_backward", dev, dc.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(da), _ptr(db), m, n, k,
           _half_flags(a), _ptr(ws), nbytes)
 
 
@@ -551,13 +552,13 @@ _BYTES = (torch.uint8,)
 
 
 def _check_mxfp4(name, q, scales):
-    """(rows, k, device) of a quantised matrix."""
+    """(rows, k, device index) of a quantised matrix."""
     rows, half = _check_first(name, q, _BYTES)
-    k, device = 2 * half, q.device
+    k, dev = 2 * half, q.get_device()
     if k % 32:
         raise ValueError("%s must hold a multiple of 32 elements per row, got %d" % (name, k))
-    _check_matrix(name + "'s scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, device)
-    return rows, k, device
+    _check_matrix(name + "'s scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, dev)
+    return rows, k, dev
 
 
 def mxfp4_quantize(x, q, scales):
@@ -566,12 +567,12 @@ def mxfp4_quantize(x, q, scales):
     The scale of 32 elements is 2 to the power floor(log2(max |x|)) - 2; elements are rounded to the nearest of 0, 0.5, 1, 1.5,
     2, 3, 4, 6 times it, ties to even codes, and magnitudes above 6 become 6.  A block with an infinity or a NaN becomes NaN."""
     rows, k = _check_first("x", x, _HALF_TYPES)
-    device = x.device
+    dev = x.get_device()
     if k % 32:
         raise ValueError("x must hold a multiple of 32 elements per row, got %d" % k)
-    _check_matrix("q", q, (rows, k // 2), torch.uint8, device)
-    _check_matrix("scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, device)
-    _call("beam_mxfp4_quantize", device, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, k, _half_flags(x))
+    _check_matrix("q", q, (rows, k // 2), torch.uint8, dev)
+    _check_matrix("scales", scales, _mxfp4_scales_shape(rows, k), torch.uint8, dev)
+    _call("beam_mxfp4_quantize", dev, x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, k, _half_flags(x))
 
 
 _MXFP4_OUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
@@ -579,23 +580,23 @@ _MXFP4_OUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 def mxfp4_dequantize(q, scales, x):
     """The values of an MXFP4 matrix in x [rows, k], float16, bfloat16 or float32 (exact in the latter two)."""
-    rows, k, device = _check_mxfp4("q", q, scales)
+    rows, k, dev = _check_mxfp4("q", q, scales)
     kind = _MXFP4_OUT.get(x.dtype) if isinstance(x, torch.Tensor) else None
-    _check_matrix("x", x, (rows, k), tuple(_MXFP4_OUT) if kind is None else x.dtype, device)
-    _call("beam_mxfp4_dequantize", device, q.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, k, kind)
+    _check_matrix("x", x, (rows, k), tuple(_MXFP4_OUT) if kind is None else x.dtype, dev)
+    _call("beam_mxfp4_dequantize", dev, q.data_ptr(), scales.data_ptr(), x.data_ptr(), rows, k, kind)
 
 
 def mxfp4_gemmrc(a, a_scales, b, b_scales, c):
     """c[M,N] = a @ b.T of two MXFP4 matrices a [M,K] and b [N,K] on the 4-bit tensor cores: fp32 accumulation, c (float16 or
     bfloat16) rounded once.  N a multiple of 8, K of 32.  Scale bytes outside the matrices must be 0, as mxfp4_quantize
     and mxfp4_tile_scales leave them."""
-    m, k, device = _check_mxfp4("a", a, a_scales)
+    m, k, dev = _check_mxfp4("a", a, a_scales)
     n = _rows(b)
-    _check_matrix("b", b, (n, k // 2), torch.uint8, device)
-    _check_matrix("b's scales", b_scales, _mxfp4_scales_shape(n, k), torch.uint8, device)
+    _check_matrix("b", b, (n, k // 2), torch.uint8, dev)
+    _check_matrix("b's scales", b_scales, _mxfp4_scales_shape(n, k), torch.uint8, dev)
     known = isinstance(c, torch.Tensor) and c.dtype in _HALF_TYPES
-    _check_matrix("c", c, (m, n), c.dtype if known else _HALF_TYPES, device)
-    _call("beam_mxfp4_gemmrc", device, a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(),
+    _check_matrix("c", c, (m, n), c.dtype if known else _HALF_TYPES, dev)
+    _call("beam_mxfp4_gemmrc", dev, a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(),
           c.data_ptr(), m, n, k, _half_flags(c))
 
 
