@@ -75,7 +75,10 @@ int launch_gated_instance(DeviceCtx* ctx, const GatedPlan& plan, int resident, c
   p.out[2] = U;
   p.status = ctx->status_word;
   p.a_rows = kCta == 2 ? S::kBM : (m + 7) / 8 * 8;
-  p.a_bytes = p.a_rows * 128;
+  // A UMMA multiplies 128 rows of A whether they exist or not.  Wide tiles keep zeros in the missing ones: with whatever lies
+  // there instead, a sustained run of one row x 16384 x 4096 is held at 1.24 GHz by the power cap (49.5 us a call, 46.8 with
+  // zeros).  Narrow tiles want their shared memory for a deeper ring (1 x 4096 x 4096: 15.7 us, 16.4 with zeros).
+  p.a_bytes = kCta == 1 && p.width < 48 ? p.a_rows * 128 : S::kABytes;
   p.stage_bytes = p.a_bytes + p.width * 128 * (kCta == 2 ? 1 : 2);
   p.m_tiles = ceil_div(m, S::kBM * kCta);
   p.n_tiles = ceil_div(f, p.width);

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
   };
 
   const uint32_t b_bytes = static_cast<uint32_t>(p.width) * 128u;
-  const uint32_t stage_tx = 2u * b_bytes + static_cast<uint32_t>(kCta) * static_cast<uint32_t>(p.a_bytes);
+  const uint32_t stage_tx = 2u * b_bytes + static_cast<uint32_t>(kCta * p.a_rows) * 128u;
   // One CTA: the loads of k-block kb into stage s (the ring of a pair: see the producers).
   auto load_stage = [&](uint32_t s, int kb, int row_a, int row_b) {
     const uint32_t a = smem_base + s * static_cast<uint32_t>(p.stage_bytes);
@@ -215,6 +215,14 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
   if (warp == 1) {
     ptx::tmem_alloc<kCta>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
     ptx::tmem_relinquish<kCta>();
+  }
+  if (kCta == 1 && p.a_bytes == S::kABytes && warp >= 2) {
+    // The rows of A that do not exist are multiplied all the same: as zeros they cost little power (see the launcher).
+    const uint32_t from = static_cast<uint32_t>(p.a_rows) * 128u;
+    for (int s = 0; s < p.stages; ++s)
+      for (uint32_t at = from + (threadIdx.x - 64u) * 16u; at < S::kABytes; at += (S::kThreads - 64u) * 16u)
+        ptx::st_shared_v4(smem_base + s * static_cast<uint32_t>(p.stage_bytes) + at, 0, 0, 0, 0);
+    ptx::fence_proxy_async_smem();
   }
   ptx::tc_fence_before();
   __syncthreads();
