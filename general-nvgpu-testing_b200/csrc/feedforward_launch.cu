@@ -106,7 +106,9 @@ int launch_gated_instance(DeviceCtx* ctx, const GatedPlan& plan, int resident, c
   const int exchange = (p.split - 1) * (p.width / p.split) * 2 * 128 * 4;  // what the others of a cluster send
   p.bar_offset = p.stages * p.stage_bytes + a_slack + S::kStagingBytes;
   if (p.bar_offset < exchange) p.bar_offset = exchange;
-  const int smem = p.bar_offset + S::kBarBytes + 1024;
+  // CTAs that wait for one another must not share an SM with CTAs of another launch that do: each of two could hold the TMEM
+  // that the other's peer waits for.  Taking all shared memory keeps such launches apart.
+  const int smem = p.split > 1 ? S::kSmemLimit : p.bar_offset + S::kBarBytes + 1024;
   const int ctas = kCta * p.split;
   return launch_dependent(gated_umma_kernel<kCta>, clusters * ctas, S::kThreads, smem, ctas, stream,
                           "cudaLaunchKernelEx(gated_umma)", p);

@@ -12,13 +12,12 @@
 //
 // Two variants, chosen by rows (the rule and what it measured stand beside gated_plan() in feedforward_launch.cu):
 //   kCta = 2   M > 128: 256-row tiles, width 32, 64, 96 or 128, persistent grid, two TMEM accumulators, C stored by TMA.
-//              4096 x 16384 x 4096 (bf16): 657 us, 1674 TFLOP/s, as fast as a cuBLAS product of that size alone; bound by
-//              the tensor pipe and the power it draws.
+//              4096 x 16384 x 4096 (bf16): 670 us, 1640 TFLOP/s, what cuBLAS takes for the two products alone (690 us); bound
+//              by the tensor pipe (94 % active), in long runs by the power it draws (1441 TFLOP/s sustained).
 //   kCta = 1   M <= 128: the call is bound by reading the weights once.  The width is whatever multiple of 8 deals F
 //              to all SMs in one wave, so that every SM streams the same share of the weights through a ring of up to 16
-//              stages; only the rows of A that exist are loaded and have room in a stage (the other lanes of the UMMA
-//              compute on what lies behind them, and are never stored); C is small and written straight from registers.
-//              One row, F = 16384, K = 4096: 45.4 us, 5.9 TB/s.  Halving the ring, so that the next launch's CTAs fit
+//              stages; only the rows of A that exist are loaded.  C is small and written straight from registers.
+//              One row, F = 16384, K = 4096: 44.5 us, 6.0 TB/s.  Halving the ring, so that the next launch's CTAs fit
 //              beside this one's, was slower for all shapes (8192 x 4096: 25.8 -> 27.8 us).
 //
 // Roles: warps 0 and 6 are TMA producers, warps 1 and 7 issue UMMAs, warps 2..5 are the epilogue.

@@ -13,9 +13,9 @@
 // have two segments, accumulated one after the other into the same tile: dA = dG Bg + dU Bu needs no second pass.
 //
 // A long list is cut into launches of whole waves.  Pairs drift apart over many tiles, and what they no longer read at the same
-// time comes from memory again: all gradients of 8192 x 16384 x 4096 read 10.8 GB in one launch against 7.8 GB in two (dA; dBg
-// and dBu), and memory traffic costs clock under the power cap.  Sustained, with all waves in one launch / 14 / 7 / 4 / 2 / 1
-// waves per launch: 3806 / 3564 / 3525 / 3516 / 3534 / 3612 us.
+// time comes from memory again: all gradients of 8192 x 16384 x 4096 read 10.8 GB in one launch and 5.1 GB in seven, and
+// memory traffic costs clock under the power cap.  Sustained, with all waves in one launch / 14 / 7 / 4 / 2 / 1 waves per
+// launch: 3806 / 3564 / 3525 / 3516 / 3534 / 3612 us; by k-blocks (see the launcher): 3512 us.
 //
 // A job with few tiles and a long contraction (dA of a short batch: M rows, but F or N steps) is cut into slices of its
 // contraction, so that it does not keep a few pairs busy while the others are done.  A slice stores its fp32 sums as a plane of

@@ -87,7 +87,9 @@ int launch_instance(DeviceCtx* ctx, const NarrowPlan& plan, int resident, const 
   if (st == BEAM_OK && kCta == 2) st = encode_tmap_2d_sw64(&p.tm_c, C, m, n, n, 32, 32);
   if (st != BEAM_OK) return st;
   const int ctas = kCta * p.split;
-  return launch_dependent(mxfp4_umma_kernel<kCta>, clusters * ctas, S::kThreads, p.bar_offset + S::kBarBytes, ctas, stream,
+  // a cluster that shares a contraction has its SMs to itself (see feedforward_launch.cu)
+  const int smem = p.split > 1 ? S::kSmemLimit : p.bar_offset + S::kBarBytes;
+  return launch_dependent(mxfp4_umma_kernel<kCta>, clusters * ctas, S::kThreads, smem, ctas, stream,
                           "cudaLaunchKernelEx(mxfp4_umma)", p);
 }
 

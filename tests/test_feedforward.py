@@ -453,6 +453,30 @@ def test_two_streams_at_once(beam, healthy):
 
 
 @pytest.mark.gpu
+def test_shared_contractions_on_two_streams(beam, healthy):
+    """Launches whose CTAs wait for one another, on two streams at once with single-CTA launches between them: all finish, and give
+    what they give alone."""
+    shapes = [(3, 512, 4096), (40, 2048, 4096), (3, 64, 512), (100, 1000, 8192)]
+    sets = [gated_inputs(m, f, k, torch.bfloat16, 7 * j) for j, (m, f, k) in enumerate(shapes)]
+    alone = []
+    for (m, f, _), s in zip(shapes, sets):
+        alone.append(torch.empty(m, f, dtype=torch.bfloat16, device="cuda"))
+        beam.gated_gemmrc(*s, alone[-1])
+    outs = [[torch.empty_like(c) for c in alone] for _ in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(50):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for j in range(len(sets)):
+                    i = (j + 2 * n) % len(sets)
+                    beam.gated_gemmrc(*sets[i], outs[n][i])
+    torch.cuda.synchronize()
+    for out in outs:
+        assert all(torch.equal(x, y) for x, y in zip(out, alone))
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_device(beam):
     a, bg, bu = gated_inputs(4, 16, 32, torch.float16)
     c = torch.empty(4, 16, dtype=torch.float16, device="cuda")
