@@ -312,7 +312,7 @@ struct GradReduceParams {
   int bf16;
 };
 
-static __global__ void __launch_bounds__(256) grad_reduce_kernel(const GradReduceParams p) {
+static __global__ void __launch_bounds__(256) grad_reduce_kernel(const __grid_constant__ GradReduceParams p) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
