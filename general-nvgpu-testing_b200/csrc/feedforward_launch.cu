@@ -250,8 +250,8 @@ int launch_grad(DeviceCtx* ctx, JobSpec* jobs, int n, int pairs, uint8_t* scratc
     if (st != BEAM_OK) return st;
     if (jobs[i].slices > 1) {
       r.planes[r.jobs] = reinterpret_cast<const float4*>(scratch);
-      r.out[r.jobs] = static_cast<uint4*>(jobs[i].c);
-      r.groups[r.jobs] = static_cast<long long>(jobs[i].rows) * (jobs[i].cols / 8);
+      r.out[r.jobs] = static_cast<uint2*>(jobs[i].c);
+      r.groups[r.jobs] = static_cast<long long>(jobs[i].rows) * (jobs[i].cols / 4);
       r.slices[r.jobs] = jobs[i].slices;
       groups += r.groups[r.jobs++];
       scratch += jobs[i].scratch_bytes();

@@ -302,11 +302,11 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
   }
 }
 
-// Adds the planes of the sliced jobs, in the order of the slices, and rounds once.  A thread does 8 columns.
+// Adds the planes of the sliced jobs, in the order of the slices, and rounds once.  A thread does 4 columns.
 struct GradReduceParams {
   const float4* planes[kMaxGradJobs];
-  uint4* out[kMaxGradJobs];
-  long long groups[kMaxGradJobs];  // of 8 elements
+  uint2* out[kMaxGradJobs];
+  long long groups[kMaxGradJobs];  // of 4 elements
   int slices[kMaxGradJobs];
   int jobs;
   int bf16;
@@ -319,17 +319,15 @@ static __global__ void __launch_bounds__(256) grad_reduce_kernel(const __grid_co
   int i = 0;
   while (i < p.jobs && at >= p.groups[i]) at -= p.groups[i++];
   if (i == p.jobs) return;
-  const long long plane = 2 * p.groups[i];
-  const float4* from = p.planes[i] + 2 * at;
-  float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-#pragma unroll 4
+  const long long plane = p.groups[i];
+  const float4* from = p.planes[i] + at;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
   for (int s = 0; s < p.slices[i]; ++s) {
-    const float4 a = __ldcs(from + s * plane), b = __ldcs(from + s * plane + 1);
-    lo.x += a.x; lo.y += a.y; lo.z += a.z; lo.w += a.w;
-    hi.x += b.x; hi.y += b.y; hi.z += b.z; hi.w += b.w;
+    const float4 a = __ldcs(from + s * plane);
+    sum.x += a.x; sum.y += a.y; sum.z += a.z; sum.w += a.w;
   }
-  p.out[i][at] = make_uint4(ptx::pack_out2(lo.x, lo.y, p.bf16), ptx::pack_out2(lo.z, lo.w, p.bf16),
-                            ptx::pack_out2(hi.x, hi.y, p.bf16), ptx::pack_out2(hi.z, hi.w, p.bf16));
+  p.out[i][at] = make_uint2(ptx::pack_out2(sum.x, sum.y, p.bf16), ptx::pack_out2(sum.z, sum.w, p.bf16));
 }
 
 }  // namespace beam
