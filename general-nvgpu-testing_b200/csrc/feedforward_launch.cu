@@ -277,7 +277,7 @@ int launch_grad(DeviceCtx* ctx, JobSpec* jobs, int n, int pairs, uint8_t* scratc
                           "cudaLaunchKernelEx(grad_umma)", p);
   }
   if (st != BEAM_OK || r.jobs == 0) return st;
-  return launch_dependent(grad_reduce_kernel, static_cast<int>((groups + 255) / 256), 256, 0, 1, stream,
+  return launch_dependent(grad_reduce_kernel, static_cast<int>((groups + 127) / 128), 128, 0, 1, stream,
                           "cudaLaunchKernelEx(grad_reduce)", r);
 }
 

@@ -312,17 +312,17 @@ struct GradReduceParams {
   int bf16;
 };
 
-static __global__ void __launch_bounds__(256) grad_reduce_kernel(const __grid_constant__ GradReduceParams p) {
+static __global__ void __launch_bounds__(128) grad_reduce_kernel(const __grid_constant__ GradReduceParams p) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  long long at = static_cast<long long>(blockIdx.x) * 128 + threadIdx.x;
   int i = 0;
   while (i < p.jobs && at >= p.groups[i]) at -= p.groups[i++];
   if (i == p.jobs) return;
   const long long plane = p.groups[i];
   const float4* from = p.planes[i] + at;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 16
   for (int s = 0; s < p.slices[i]; ++s) {
     const float4 a = __ldcs(from + s * plane);
     sum.x += a.x; sum.y += a.y; sum.z += a.z; sum.w += a.w;
