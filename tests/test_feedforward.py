@@ -157,8 +157,10 @@ def test_c_entries_refuse_bad_arguments(built_library):
     need = L.beam_gated_gemmrc_backward_workspace_bytes
     need.restype, need.argtypes = sz, [i, i, i]
     assert need(64, 64, 64) == 2 * 64 * 64 * 2 and need(3, 8, 64) == 2 * 256 and need(0, 8, 8) == 0
-    # 74 pairs without a device: dA of 16 rows is 4 tiles of 512 k-blocks, the weights' 512 tiles of one: 34 k-blocks per pair
-    assert need(16, 16384, 1024) == 2 * 16 * 16384 * 2 + 512 // 35 * 16 * 1024 * 4
+    # 74 pairs without a device: dA of 16 rows is 4 tiles of 512 k-blocks, in the most slices that there are
+    assert need(16, 16384, 1024) == 2 * 16 * 16384 * 2 + 16 * 16 * 1024 * 4
+    # 8 tiles of 86 k-blocks in 7 slices and 88 tiles of 6 are 144 items, two rounds of 74 pairs
+    assert need(333, 2744, 1000) == 2 * (-(-333 * 2744 * 2 // 256) * 256) + -(-7 * 333 * 1000 * 4 // 256) * 256
     f = L.beam_gated_gemmrc_backward
     f.argtypes = [vp] * 9 + [i, i, i, i, i, vp, sz, vp]
     good = p[:9] + [64, 64, 64, 1, 2, p[9], need(64, 64, 64), None]
@@ -175,8 +177,8 @@ def test_c_entries_refuse_bad_arguments(built_library):
     need = L.beam_gemmrc_backward_workspace_bytes
     need.restype, need.argtypes = sz, [i, i, i]
     assert need(64, 64, 64) == 0 and need(8192, 4096, 8192) == 0 and need(64, 60, 64) == 0
-    # dA is one tile of 64 k-blocks, in slices of 8; dB 16 tiles of one k-block
-    assert need(64, 4096, 256) == 8 * 64 * 256 * 4
+    # dA is one tile of 64 k-blocks, in slices of 4; dB 16 tiles of one k-block
+    assert need(64, 4096, 256) == 16 * 64 * 256 * 4
     f = L.beam_gemmrc_backward
     f.argtypes = [vp] * 5 + [i, i, i, i, vp, sz, vp]
     good = p[:5] + [64, 64, 64, 0, None, 0, None]
