@@ -128,10 +128,7 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
       ptx::mbar_init(tmem_empty_bar(lane), 8);  // one arrive per epilogue warp of each CTA
     }
     ptx::fence_mbar_init();
-    if (lane == 0) {
-      *cta_abort = 0;
-      ptx::grid_launch_dependents();
-    }
+    if (lane == 0) *cta_abort = 0;
     __syncwarp();
   }
   if (warp == 1) {
@@ -143,10 +140,10 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
   ptx::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  enter_stream_order(warp);
 
   if (warp == 0 || warp == 6) {
     // ------------------------------------------------------------------ TMA producers
-    ptx::grid_dependency_wait();  // before the first global read
     const bool left = warp == 0;
     uint32_t s = 0, ph = 0;
     bool alive = true;
@@ -318,8 +315,8 @@ struct GradReduceParams {
 };
 
 static __global__ void __launch_bounds__(128) grad_reduce_kernel(const __grid_constant__ GradReduceParams p) {
-  ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();  // see enter_stream_order()
   long long at = static_cast<long long>(blockIdx.x) * 128 + threadIdx.x;
   int i = 0;
   while (i < p.jobs && at >= p.groups[i]) at -= p.groups[i++];

@@ -60,8 +60,8 @@ struct MxQuantParams {
 
 template <bool kBf16>
 static __global__ void __launch_bounds__(256, 8) mxfp4_quantize_kernel(const MxQuantParams p) {
-  ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();  // see enter_stream_order()
   const MxPlace at = mx_place(p.units);
   const bool in_k = at.col < static_cast<uint32_t>(p.k);
   const size_t first = (static_cast<size_t>(at.row) * p.k + at.col) >> 3, step = (static_cast<size_t>(at.step) * p.k) >> 3;
@@ -109,8 +109,8 @@ template <int kType>
 static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* __restrict__ q,
                                                                       const uint8_t* __restrict__ scales,
                                                                       uint4* __restrict__ x, int k, MxUnits units) {
-  ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();  // see enter_stream_order()
   const MxPlace at = mx_place(units);
   if (at.col >= static_cast<uint32_t>(k)) return;
   const size_t first = (static_cast<size_t>(at.row) * k + at.col) >> 3, step = (static_cast<size_t>(at.step) * k) >> 3;
@@ -329,7 +329,6 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
       ptx::prefetch_tensormap(&p.tm_b);
       ptx::prefetch_tensormap(&p.tm_sa);
       ptx::prefetch_tensormap(&p.tm_sb);
-      ptx::grid_launch_dependents();
     }
     __syncwarp();
     if constexpr (kCta == 1) {
@@ -359,11 +358,11 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
   if constexpr (kCta == 2) ptx::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  enter_stream_order(warp);
 
   if (warp == 0 || warp == S::kSecondProducer) {
     // ------------------------------------------------------------------ TMA producers
     const bool left = warp == 0;
-    ptx::grid_dependency_wait();  // before the first global read
     const uint32_t stages = static_cast<uint32_t>(p.stages);
     int kb = preloaded;  // at most the ring
     uint32_t s = static_cast<uint32_t>(kb) % stages, ph = static_cast<uint32_t>(kb) / stages;

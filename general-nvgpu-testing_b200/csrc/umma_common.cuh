@@ -92,6 +92,18 @@ __device__ __forceinline__ bool bounded_wait_converged(uint32_t bar, uint32_t pa
   return ok;
 }
 
+// A kernel's place among its neighbours on the stream, taken by every warp once the CTA (pair) is set up and has its TMEM: it
+// waits for the kernel before it, and only then lets the kernel behind it start.  The order matters three times.
+//   * A kernel that starts has the one before its predecessor complete behind it.  A split-K call whose caller vouches for its
+//     inputs (BEAM_FLAG_INPUTS_STABLE) reads them without a wait, so this is what that promise rests on.
+//   * CTAs of the kernel behind may share an SM with this one's where shared memory allows (narrow gated products take 64 KB).  Let
+//     in before this CTA had its TMEM, they could take it and then wait for this grid, which would wait for them.
+//   * No role begins a bounded wait while the kernel before is still at work, however long that takes.
+__device__ __forceinline__ void enter_stream_order(uint32_t warp) {
+  ptx::grid_dependency_wait();
+  if (warp == 0) ptx::grid_launch_dependents();
+}
+
 // ---- joining the sums of a contraction that the CTAs of a cluster have split among them
 // Every CTA holds the sums over its own share of K, fp32 in TMEM.  Each finishes one slice of the columns: it sends the others'
 // slices into their shared memory (their rings are idle by then) and adds what arrives to its own.  What one source sends is

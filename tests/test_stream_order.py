@@ -1,0 +1,140 @@
+"""Kernels that are launched as programmatic dependents and their place on the stream.
+
+A kernel may start before the one ahead of it has finished.  What keeps results right is an order inside every kernel: it waits
+for the kernel ahead (griddepcontrol.wait), and only then lets the one behind start (griddepcontrol.launch_dependents); and a
+CTA that needs TMEM has it by then.  A violation is a race between kernels, so the order is read from the sources here, on
+the CPU; the GPU tests run chains of calls in which a violation would show.
+"""
+import glob
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+WAIT, RELEASE, ALLOC = "ptx::grid_dependency_wait()", "ptx::grid_launch_dependents()", "ptx::tmem_alloc<"
+# Split-K kernels let the next call stream beside them on purpose; BEAM_FLAG_INPUTS_STABLE says what a caller vouches for.
+SPLIT_K = {"splitk_stream_kernel", "splitk_reduce_kernel", "splitk_reduce_flat_kernel", "gemmrc_umma_kernel"}
+FEED_FORWARD = ("gated_umma.cuh", "grad_umma.cuh", "mxfp4_umma.cuh")
+
+
+def bare(text):
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def kernels(path):
+    """name -> body of every kernel of a file, with calls of enter_stream_order() spelled out."""
+    with open(os.path.join(ROOT, "general-nvgpu-testing_b200", "csrc", "umma_common.cuh")) as f:
+        common = bare(f.read())
+    order = re.search(r"void enter_stream_order\(uint32_t warp\) \{(.*?)\n\}", common, re.S)
+    order = order.group(1) if order else ""
+    with open(path) as f:
+        text = bare(f.read())
+    found = {}
+    for m in re.finditer(r"__global__ void __launch_bounds__\([^\n]*\)\s+(\w+)\(", text):
+        start = text.index("{", m.end())
+        depth, at = 1, start + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[at], 0)
+            at += 1
+        found[m.group(1)] = text[start:at].replace("enter_stream_order(warp);", order)
+    return found
+
+
+def sources():
+    return sorted(glob.glob(os.path.join(ROOT, "general-nvgpu-testing_b200", "csrc", "*.cuh")))
+
+
+def test_the_sources_are_understood():
+    names = {n for p in sources() for n in kernels(p)}
+    assert {"gated_umma_kernel", "gated_slope_kernel", "grad_umma_kernel", "grad_reduce_kernel", "mxfp4_quantize_kernel",
+            "mxfp4_dequantize_kernel", "mxfp4_umma_kernel"} | SPLIT_K <= names
+
+
+@pytest.mark.parametrize("name", FEED_FORWARD)
+def test_dependents_are_released_after_the_wait_and_the_tmem(name):
+    path = os.path.join(ROOT, "general-nvgpu-testing_b200", "csrc", name)
+    for kernel, body in kernels(path).items():
+        assert body.count(RELEASE) == 1, kernel
+        release = body.index(RELEASE)
+        assert 0 <= body.find(WAIT) < release, kernel + " lets the next kernel start before it has waited itself"
+        if ALLOC in body:
+            barrier = body.index("__syncthreads()", body.index(ALLOC))
+            assert barrier < release, kernel + " lets the next kernel start before it has its TMEM"
+            # every role of the kernel waits: the wait directly ahead of the release is outside all branches on the warp
+            assert re.search(r"tmem_base = \*tmem_slot;\s*" + re.escape(WAIT), body), kernel
+
+
+@pytest.fixture(scope="module")
+def beam(built_library):
+    import beam as beam_pkg
+    return beam_pkg
+
+
+def normal(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("between", ("quantize", "dequantize", "gradient", "product"))
+def test_split_k_on_the_result_of_the_call_before_the_last(beam, between):
+    """A gated product, a small call on other tensors, then a split-K call on the gated result that vouches for its inputs: they
+    are not outputs of the call just before it."""
+    m, f, k = 96, 32768, 2048
+    a, bg, bu = (normal(s, torch.float16, j, c) for j, (s, c) in enumerate((((m, k), 1.0), ((f, k), k ** -0.5), ((f, k), k ** -0.5))))
+    w = normal((64, f), torch.float16, 5, f ** -0.5)
+    h, want_h = (torch.empty(m, f, dtype=torch.float16, device="cuda") for _ in range(2))
+    c, want_c = (torch.empty(m, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    x = normal((8, 256), torch.float16, 7)
+    v, dx = torch.empty_like(x), torch.empty_like(x)
+    q, y = beam.mxfp4_empty(8, 256), torch.empty(8, 8, dtype=torch.float16, device="cuda")
+    beam.mxfp4_quantize(x, *q)
+    beam.gated_gemmrc(a, bg, bu, want_h)
+    torch.cuda.synchronize()
+    beam.cutlass_gemmrc_splitk(want_h, w, want_c)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        h.zero_()
+        c.zero_()
+        beam.gated_gemmrc(a, bg, bu, h)
+        if between == "quantize":
+            beam.mxfp4_quantize(x, *q)
+        elif between == "dequantize":
+            beam.mxfp4_dequantize(*q, v)
+        elif between == "gradient":
+            beam.gemmrc_backward(y, x, x, da=dx)
+        else:
+            beam.mxfp4_gemmrc(*q, *q, y)
+        beam.cutlass_gemmrc_splitk(h, w, c, inputs_stable=True)
+        # the split factor differs from the plain call's, and with it the order of the sums: at most 512 partial sums per element,
+        # each off by 2^-23 of sum |h w|, and the two roundings to fp16
+        size = want_h.double().abs() @ w.double().abs().t()
+        tol = 2.0 ** -10 * want_c.double().abs() + (f / 16 + 512) * 2.0 ** -22 * size + 2.0 ** -24
+        assert ((c.double() - want_c.double()).abs() <= tol).all()
+    assert beam.device_status() == (0, 0)
+
+
+@pytest.mark.gpu
+def test_long_chains_of_small_calls(beam):
+    """Narrow gated products take little shared memory: several of a chain's CTAs fit on one SM, and each needs all of its TMEM.  The
+    chain finishes, and every call sees the result of the one before."""
+    d, t = 512, torch.bfloat16
+    # element 0 stays 1 and is every element's gate; the others are turned by an orthogonal matrix
+    gate, up = torch.zeros(2, d, d, dtype=t, device="cuda")
+    gate[:, 0] = 1
+    up[0, 0] = 1
+    up[1:, 1:] = torch.linalg.qr(normal((d - 1, d - 1), torch.float64, 10))[0].to(t)
+    x = [normal((1, d), t, 20)] + [torch.full((1, d), float("nan"), dtype=t, device="cuda") for _ in range(200)]
+    x[0][0, 0] = 1
+    for j in range(200):
+        beam.gated_gemmrc(x[j], gate, up, x[j + 1], activation="relu")
+    torch.cuda.synchronize()
+    assert beam.device_status() == (0, 0)
+    for j in range(200):  # each call again, alone
+        c = torch.empty_like(x[0])
+        beam.gated_gemmrc(x[j], gate, up, c, activation="relu")
+        torch.cuda.synchronize()
+        assert torch.equal(c, x[j + 1]), j
+    assert x[200][0, 0] == 1 and 0.5 < x[200].float().norm() / x[0].float().norm() < 2  # nothing has died out on the way
