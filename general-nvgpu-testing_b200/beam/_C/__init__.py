@@ -291,8 +291,9 @@ def _splitk(a, b, c, tile_n, split_k_slices, inputs_stable, two_kernels=None):
 def cutlass_gemmrc_splitk(a, b, c, split_k_slices=0, inputs_stable=False, two_kernels=None):
     """Split-K c = a @ b.T for small M, N and huge K; fp32 partials summed in a fixed order (bitwise
     reproducible).  split_k_slices = 0 lets the library choose (slot of cutlass_gemmrc_splitk.cu:59-105).
-    inputs_stable=True promises that a and b are not outputs of the kernel just before this call on the
-    stream, which lets back-to-back calls overlap (BEAM_FLAG_INPUTS_STABLE).  two_kernels=True forces the
+    inputs_stable=True promises that a and b are not outputs of the call just before this one on the stream
+    (in a run of calls with inputs_stable=True: of none in the run, nor of the call just before the run), which
+    lets back-to-back calls overlap (BEAM_FLAG_INPUTS_STABLE).  two_kernels=True forces the
     partials-then-reduction pair of kernels where the library would run the call as one kernel, False the one-kernel
     form where the library would launch two (same bits either way); None leaves the choice to the library."""
     _splitk(a, b, c, 0, split_k_slices, inputs_stable, two_kernels)

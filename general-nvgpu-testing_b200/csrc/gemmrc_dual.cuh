@@ -94,10 +94,6 @@ __global__ void __launch_bounds__((DualShape<kStages, kCta>::kThreads), 1) gemmr
     ptx::prefetch_tensormap(&p.tm_a);
     ptx::prefetch_tensormap(&p.tm_b);
     ptx::prefetch_tensormap(&p.tm_c);
-    // A programmatic dependent of the kernel before it on the stream: the whole set-up may overlap that kernel's last
-    // CTAs; the two producer threads wait for that grid before their first load, and nothing is written before data
-    // has arrived.
-    ptx::grid_launch_dependents();
   }
   if (warp == 1) {
     ptx::tmem_alloc<kCta>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
@@ -108,11 +104,12 @@ __global__ void __launch_bounds__((DualShape<kStages, kCta>::kThreads), 1) gemmr
   if constexpr (kCta == 2) ptx::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // A programmatic dependent of the kernel before it on the stream: everything above may overlap that kernel's last CTAs.
+  enter_stream_order(warp);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      ptx::grid_dependency_wait();
       uint32_t it = 0;
       bool alive = true;
       const uint64_t pol_a = ptx::l2_policy(p.hint_a);
@@ -148,7 +145,6 @@ __global__ void __launch_bounds__((DualShape<kStages, kCta>::kThreads), 1) gemmr
     // with the B box on a thread of its own the kernel gains 1.7 % (one CTA per tile) and 3.5 % (pairs) at 8192^3
     // (a thread per box is slower again).  Both producers walk the same items and wait on the same empty barriers.
     if (lane == 0) {
-      ptx::grid_dependency_wait();
       uint32_t it = 0;
       bool alive = true;
       const uint64_t pol_b = ptx::l2_policy(p.hint_b);

@@ -97,8 +97,6 @@ __global__ void __launch_bounds__(192, 2) splitk_stream_kernel(const __grid_cons
     ptx::prefetch_tensormap(&p.tm_b);
     ptx::prefetch_tensormap(&p.tm_s);
     ptx::prefetch_tensormap(&p.tm_peer[0]);
-    // The next kernel on the stream may become resident now; it blocks in its own griddepcontrol.wait.
-    ptx::grid_launch_dependents();
   }
   if (warp == 1) {
     ptx::tmem_alloc<1>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
@@ -108,6 +106,12 @@ __global__ void __launch_bounds__(192, 2) splitk_stream_kernel(const __grid_cons
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (warp == 2 && lane == 0) {
+    // The next kernel on the stream may become resident now; it blocks in its own griddepcontrol.wait.  Whoever vouches for
+    // that kernel's inputs relies on this call having waited (see enter_stream_order()), unless it was vouched for as well.
+    if (!(p.flags & 1)) ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+  }
 
   // ---- this CTA's work item: slice fastest, then N tile, then M tile
   const int num_kb = kFold ? ((p.k + S::kBK - 1) / S::kBK + 1) / 2 : (p.k + S::kBK - 1) / S::kBK;

@@ -66,11 +66,13 @@ typedef struct beam_gemm_cfg {
                          the wait for its predecessor's result); 1 = one tile at a time                     */
 } beam_gemm_cfg;
 
-/* Split-K only.  The caller guarantees that A and B are not outputs of the kernel that immediately precedes
- * this call on the stream (they were complete before that kernel started).  The first kernel of the call is
- * a programmatic dependent launch; with this flag it starts streaming A and B while the preceding kernel
- * (typically the previous split-K call's reduction) is still finishing, and only its writes wait for that
- * kernel to complete.  Without the flag it waits before its first global read, which is always safe. */
+/* Split-K only.  The caller guarantees that A and B are not outputs of the call (or other kernel) that immediately
+ * precedes this one on the stream; where that is a split-K call with this flag too, not of the one before it either, and
+ * so on back to the last one without the flag, included.  The first kernel of the call is a programmatic dependent launch;
+ * with this flag it starts streaming A and B while the preceding kernel (typically the previous split-K call's reduction)
+ * is still finishing, and only its writes wait for that kernel to complete.  Every other call of this library waits for
+ * what precedes it before it lets the next call start, so what was queued before those calls is complete by then.
+ * Without the flag the call waits before its first global read, which is always safe. */
 #define BEAM_FLAG_INPUTS_STABLE 1
 /* beam_gemmrc_fp16 only: A, B and C hold bf16 instead of fp16 (same kernels; fp32 accumulation, one rounding to
  * bf16).  The reference reaches bf16 only through its cuBLAS comparator (cuda/cublas.cc:106-108). */

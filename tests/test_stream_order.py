@@ -16,7 +16,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 WAIT, RELEASE, ALLOC = "ptx::grid_dependency_wait()", "ptx::grid_launch_dependents()", "ptx::tmem_alloc<"
 # Split-K kernels let the next call stream beside them on purpose; BEAM_FLAG_INPUTS_STABLE says what a caller vouches for.
 SPLIT_K = {"splitk_stream_kernel", "splitk_reduce_kernel", "splitk_reduce_flat_kernel", "gemmrc_umma_kernel"}
-FEED_FORWARD = ("gated_umma.cuh", "grad_umma.cuh", "mxfp4_umma.cuh")
+ORDERED = ("gated_umma.cuh", "grad_umma.cuh", "mxfp4_umma.cuh", "gemmrc_dual.cuh", "gemmrc_wide.cuh")
 
 
 def bare(text):
@@ -52,7 +52,7 @@ def test_the_sources_are_understood():
             "mxfp4_dequantize_kernel", "mxfp4_umma_kernel"} | SPLIT_K <= names
 
 
-@pytest.mark.parametrize("name", FEED_FORWARD)
+@pytest.mark.parametrize("name", ORDERED)
 def test_dependents_are_released_after_the_wait_and_the_tmem(name):
     path = os.path.join(ROOT, "general-nvgpu-testing_b200", "csrc", name)
     for kernel, body in kernels(path).items():
@@ -64,6 +64,23 @@ def test_dependents_are_released_after_the_wait_and_the_tmem(name):
             assert barrier < release, kernel + " lets the next kernel start before it has its TMEM"
             # every role of the kernel waits: the wait directly ahead of the release is outside all branches on the warp
             assert re.search(r"tmem_base = \*tmem_slot;\s*" + re.escape(WAIT), body), kernel
+
+
+def test_split_k_kernels_wait_before_they_release():
+    """... unless the caller vouches for the inputs.  The kernel that leaves room on its SM has its TMEM by then, and the one that
+    split-K shares with the plain product keeps the whole order for the latter."""
+    seen = {}
+    for path in sources():
+        seen.update({n: b for n, b in kernels(path).items() if n in SPLIT_K and ALLOC in b})
+    assert set(seen) == {"splitk_stream_kernel", "gemmrc_umma_kernel"}
+    for kernel, body in seen.items():
+        assert 0 <= body.find(WAIT) < body.index(RELEASE), kernel
+    body = seen["splitk_stream_kernel"]
+    assert body.index("__syncthreads()", body.index(ALLOC)) < body.index(RELEASE)
+    body = seen["gemmrc_umma_kernel"]
+    first, last = (m.start() for m in re.finditer(re.escape(RELEASE), body))
+    assert body[:first].rstrip().endswith("if constexpr (is_splitk_mode(kMode))")
+    assert body.index("__syncthreads()", body.index(ALLOC)) < body.index("if constexpr (kMode == kModeGemm)") < last
 
 
 @pytest.fixture(scope="module")
@@ -78,7 +95,7 @@ def normal(shape, dtype, seed, scale=1.0):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("between", ("quantize", "dequantize", "gradient", "product"))
+@pytest.mark.parametrize("between", ("quantize", "dequantize", "gradient", "product", "plain", "one plain kernel"))
 def test_split_k_on_the_result_of_the_call_before_the_last(beam, between):
     """A gated product, a small call on other tensors, then a split-K call on the gated result that vouches for its inputs: they
     are not outputs of the call just before it."""
@@ -105,6 +122,10 @@ def test_split_k_on_the_result_of_the_call_before_the_last(beam, between):
             beam.mxfp4_dequantize(*q, v)
         elif between == "gradient":
             beam.gemmrc_backward(y, x, x, da=dx)
+        elif between == "plain":
+            beam.gemmrc(x, x, y)
+        elif between == "one plain kernel":
+            beam.cutlass_gemmrc_splitk(x, x, y, two_kernels=False)
         else:
             beam.mxfp4_gemmrc(*q, *q, y)
         beam.cutlass_gemmrc_splitk(h, w, c, inputs_stable=True)
