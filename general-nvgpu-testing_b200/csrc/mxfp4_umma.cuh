@@ -106,9 +106,8 @@ enum MxType : int { kMxFp16 = 0, kMxBf16 = 1, kMxFp32 = 2 };
 
 // The inverse: x = q 2^s, exact in fp32 and rounded to the output type.  Same units.
 template <int kType>
-static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* __restrict__ q,
-                                                                      const uint8_t* __restrict__ scales,
-                                                                      uint4* __restrict__ x, int k, MxUnits units) {
+static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* q, const uint8_t* scales, uint4* x,
+                                                                      int k, MxUnits units) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();  // see enter_stream_order()
   const MxPlace at = mx_place(units);
@@ -122,7 +121,7 @@ static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint
     code[i] = byte[i] = 0;
     if (row < static_cast<uint32_t>(units.rows)) {
       code[i] = __ldcs(q + first + i * step);
-      byte[i] = __ldg(scales + mx_scale_row(row));
+      byte[i] = __ldcg(scales + mx_scale_row(row));  // no read-only path: the kernel ahead may have written them since this one began
     }
   }
 #pragma unroll

@@ -66,6 +66,15 @@ def test_dependents_are_released_after_the_wait_and_the_tmem(name):
             assert re.search(r"tmem_base = \*tmem_slot;\s*" + re.escape(WAIT), body), kernel
 
 
+@pytest.mark.parametrize("name", ORDERED)
+def test_no_read_only_loads(name):
+    """A load through the read-only path may return what the memory held when the kernel began; its inputs may be written after that, by
+    the kernel ahead."""
+    with open(os.path.join(ROOT, "general-nvgpu-testing_b200", "csrc", name)) as f:
+        text = bare(f.read())
+    assert "__ldg(" not in text and ".nc" not in text and "__restrict__" not in text
+
+
 def test_split_k_kernels_wait_before_they_release():
     """... unless the caller vouches for the inputs.  The kernel that leaves room on its SM has its TMEM by then, and the one that
     split-K shares with the plain product keeps the whole order for the latter."""
@@ -135,6 +144,28 @@ def test_split_k_on_the_result_of_the_call_before_the_last(beam, between):
         tol = 2.0 ** -10 * want_c.double().abs() + (f / 16 + 512) * 2.0 ** -22 * size + 2.0 ** -24
         assert ((c.double() - want_c.double()).abs() <= tol).all()
     assert beam.device_status() == (0, 0)
+
+
+@pytest.mark.gpu
+def test_values_follow_their_quantisation(beam):
+    """Quantise and dequantise through the same small tensors again and again: every call returns the values of the latest codes and
+    scales."""
+    xs = [normal((130, 160), torch.bfloat16, j, 4.0 ** (j - 4)) for j in range(8)]
+    codes, alone = beam.mxfp4_empty(130, 160), []
+    for x in xs:
+        q = beam.mxfp4_empty(130, 160)
+        beam.mxfp4_quantize(x, *q)
+        torch.cuda.synchronize()
+        alone.append(torch.empty(130, 160, device="cuda"))
+        beam.mxfp4_dequantize(*q, alone[-1])
+        torch.cuda.synchronize()
+    seen = [[torch.empty_like(v) for v in alone] for _ in range(25)]
+    for out in seen:
+        for x, v in zip(xs, out):
+            beam.mxfp4_quantize(x, *codes)
+            beam.mxfp4_dequantize(*codes, v)
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want) for out in seen for v, want in zip(out, alone))
 
 
 @pytest.mark.gpu
