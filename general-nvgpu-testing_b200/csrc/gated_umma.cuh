@@ -227,10 +227,11 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
   if constexpr (kCta == 2) ptx::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  enter_stream_order(warp);
+  release_next_kernel(warp);
 
   if (warp == 0 || (warp >= 6 && warp < S::kSecondIssuer)) {
     // ------------------------------------------------------------------ TMA producers
+    ptx::grid_dependency_wait();  // before the first global read; everything else follows from these reads
     const uint32_t mine = warp == 0 ? 0u : warp - 5u;  // this warp fills every kProducers-th stage of the walk
     const uint32_t stages = static_cast<uint32_t>(p.stages);
     const CUtensorMap* tm_b = leader ? &p.tm_gate : &p.tm_up;
@@ -490,7 +491,7 @@ __device__ __forceinline__ void gated_slope8(const uint4& d4, const uint4& g4, c
 template <int kAct, bool kBf16>
 __global__ void __launch_bounds__(256) gated_slope_kernel(const GatedSlopeParams p) {
   ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();  // see enter_stream_order()
+  ptx::grid_launch_dependents();  // see release_next_kernel()
   const long long stride = static_cast<long long>(gridDim.x) * 256;
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < p.count8; i += stride) {
     uint4 dg, du;

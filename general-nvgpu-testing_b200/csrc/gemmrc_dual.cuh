@@ -105,11 +105,12 @@ __global__ void __launch_bounds__((DualShape<kStages, kCta>::kThreads), 1) gemmr
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // A programmatic dependent of the kernel before it on the stream: everything above may overlap that kernel's last CTAs.
-  enter_stream_order(warp);
+  release_next_kernel(warp);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
+      ptx::grid_dependency_wait();  // the preceding grid has completed: A and B may be its outputs
       uint32_t it = 0;
       bool alive = true;
       const uint64_t pol_a = ptx::l2_policy(p.hint_a);
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__((DualShape<kStages, kCta>::kThreads), 1) gemmr
     // with the B box on a thread of its own the kernel gains 1.7 % (one CTA per tile) and 3.5 % (pairs) at 8192^3
     // (a thread per box is slower again).  Both producers walk the same items and wait on the same empty barriers.
     if (lane == 0) {
+      ptx::grid_dependency_wait();
       uint32_t it = 0;
       bool alive = true;
       const uint64_t pol_b = ptx::l2_policy(p.hint_b);

@@ -507,11 +507,12 @@ __global__ void __launch_bounds__((GemmShape<BN, kStages, kCta, kMode>::kThreads
   if constexpr (kCta == 2) ptx::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  if constexpr (kMode == kModeGemm) enter_stream_order(warp);
+  if constexpr (kMode == kModeGemm) release_next_kernel(warp);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
+      if constexpr (kMode == kModeGemm && kCta == 2) ptx::grid_dependency_wait();  // before the first global read
       uint32_t it = 0;
       bool alive = true;
       const uint64_t pol_a = ptx::l2_policy(p.hint_a);

@@ -100,14 +100,15 @@ __global__ void __launch_bounds__(WideShape<kStages>::kThreads, 1) gemmrc_wide_k
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // Launched as a programmatic dependent of the kernel before it on the stream: this CTA may have become resident and run
-  // the set-up above while that kernel's last CTAs were still at work.  From here on that grid has completed (A and B may be
-  // its outputs), and the next kernel on the stream may take SMs as this grid's CTAs leave them.
-  enter_stream_order(warp);
+  // the set-up above while that kernel's last CTAs were still at work.  The producer thread waits for that grid before its first
+  // load; nothing is written before data arrives.  In turn, the next kernel may take SMs as this grid's CTAs leave them.
+  release_next_kernel(warp);
   const int num_kb = (p.k + S::kBK - 1) / S::kBK;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
+      ptx::grid_dependency_wait();  // the preceding grid has completed: A and B may be its outputs
       uint32_t it = 0;
       bool alive = true;
       const uint64_t pol_a = ptx::l2_policy(p.hint_a);

@@ -140,10 +140,11 @@ static __global__ void __launch_bounds__(GradShape::kThreads, 1) grad_umma_kerne
   ptx::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  enter_stream_order(warp);
+  release_next_kernel(warp);
 
   if (warp == 0 || warp == 6) {
     // ------------------------------------------------------------------ TMA producers
+    ptx::grid_dependency_wait();  // before the first global read
     const bool left = warp == 0;
     uint32_t s = 0, ph = 0;
     bool alive = true;
@@ -316,7 +317,7 @@ struct GradReduceParams {
 
 static __global__ void __launch_bounds__(128) grad_reduce_kernel(const __grid_constant__ GradReduceParams p) {
   ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();  // see enter_stream_order()
+  ptx::grid_launch_dependents();  // see release_next_kernel()
   long long at = static_cast<long long>(blockIdx.x) * 128 + threadIdx.x;
   int i = 0;
   while (i < p.jobs && at >= p.groups[i]) at -= p.groups[i++];

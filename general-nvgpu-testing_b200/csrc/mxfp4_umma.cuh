@@ -61,7 +61,7 @@ struct MxQuantParams {
 template <bool kBf16>
 static __global__ void __launch_bounds__(256, 8) mxfp4_quantize_kernel(const MxQuantParams p) {
   ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();  // see enter_stream_order()
+  ptx::grid_launch_dependents();  // see release_next_kernel()
   const MxPlace at = mx_place(p.units);
   const bool in_k = at.col < static_cast<uint32_t>(p.k);
   const size_t first = (static_cast<size_t>(at.row) * p.k + at.col) >> 3, step = (static_cast<size_t>(at.step) * p.k) >> 3;
@@ -109,7 +109,7 @@ template <int kType>
 static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* q, const uint8_t* scales, uint4* x,
                                                                       int k, MxUnits units) {
   ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();  // see enter_stream_order()
+  ptx::grid_launch_dependents();  // see release_next_kernel()
   const MxPlace at = mx_place(units);
   if (at.col >= static_cast<uint32_t>(k)) return;
   const size_t first = (static_cast<size_t>(at.row) * k + at.col) >> 3, step = (static_cast<size_t>(at.step) * k) >> 3;
@@ -357,11 +357,12 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
   if constexpr (kCta == 2) ptx::cluster_sync_all();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  enter_stream_order(warp);
+  release_next_kernel(warp);
 
   if (warp == 0 || warp == S::kSecondProducer) {
     // ------------------------------------------------------------------ TMA producers
     const bool left = warp == 0;
+    ptx::grid_dependency_wait();  // before the first global read
     const uint32_t stages = static_cast<uint32_t>(p.stages);
     int kb = preloaded;  // at most the ring
     uint32_t s = static_cast<uint32_t>(kb) % stages, ph = static_cast<uint32_t>(kb) / stages;

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(192, 2) splitk_stream_kernel(const __grid_cons
   const uint32_t tmem_base = *tmem_slot;
   if (warp == 2 && lane == 0) {
     // The next kernel on the stream may become resident now; it blocks in its own griddepcontrol.wait.  Whoever vouches for
-    // that kernel's inputs relies on this call having waited (see enter_stream_order()), unless it was vouched for as well.
+    // that kernel's inputs relies on this call having waited (see release_next_kernel()), unless it was vouched for as well.
     if (!(p.flags & 1)) ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
   }

@@ -24,11 +24,11 @@ def bare(text):
 
 
 def kernels(path):
-    """name -> body of every kernel of a file, with calls of enter_stream_order() spelled out."""
+    """name -> body of every kernel of a file, with calls of release_next_kernel() spelled out."""
     with open(os.path.join(ROOT, "general-nvgpu-testing_b200", "csrc", "umma_common.cuh")) as f:
         common = bare(f.read())
-    order = re.search(r"void enter_stream_order\(uint32_t warp\) \{(.*?)\n\}", common, re.S)
-    order = order.group(1) if order else ""
+    release = re.search(r"void release_next_kernel\(uint32_t warp\) \{(.*?)\n\}", common, re.S)
+    release = release.group(1) if release else ""
     with open(path) as f:
         text = bare(f.read())
     found = {}
@@ -38,7 +38,7 @@ def kernels(path):
         while depth:
             depth += {"{": 1, "}": -1}.get(text[at], 0)
             at += 1
-        found[m.group(1)] = text[start:at].replace("enter_stream_order(warp);", order)
+        found[m.group(1)] = text[start:at].replace("release_next_kernel(warp);", release)
     return found
 
 
@@ -58,12 +58,20 @@ def test_dependents_are_released_after_the_wait_and_the_tmem(name):
     for kernel, body in kernels(path).items():
         assert body.count(RELEASE) == 1, kernel
         release = body.index(RELEASE)
-        assert 0 <= body.find(WAIT) < release, kernel + " lets the next kernel start before it has waited itself"
+        # the same threads wait directly ahead of it
+        assert body[:release].rstrip().endswith(WAIT + ";"), kernel + " lets the next kernel start before it has waited itself"
         if ALLOC in body:
             barrier = body.index("__syncthreads()", body.index(ALLOC))
             assert barrier < release, kernel + " lets the next kernel start before it has its TMEM"
-            # every role of the kernel waits: the wait directly ahead of the release is outside all branches on the warp
-            assert re.search(r"tmem_base = \*tmem_slot;\s*" + re.escape(WAIT), body), kernel
+
+
+def test_bounded_waits_begin_when_the_kernel_ahead_has_finished():
+    with open(os.path.join(ROOT, "general-nvgpu-testing_b200", "csrc", "umma_common.cuh")) as f:
+        common = bare(f.read())
+    for name in ("bool bounded_wait(", "bool bounded_wait_warp("):
+        body = common[common.index(name):]
+        body = body[:body.index("\n}")]
+        assert re.search(r"if \(t0 == 0\) " + re.escape(WAIT) + r";\s*const uint64_t now = ptx::globaltimer_ns\(\);", body), name
 
 
 @pytest.mark.parametrize("name", ORDERED)
@@ -144,6 +152,40 @@ def test_split_k_on_the_result_of_the_call_before_the_last(beam, between):
         tol = 2.0 ** -10 * want_c.double().abs() + (f / 16 + 512) * 2.0 ** -22 * size + 2.0 ** -24
         assert ((c.double() - want_c.double()).abs() <= tol).all()
     assert beam.device_status() == (0, 0)
+
+
+@pytest.mark.gpu
+def test_behind_a_call_of_several_seconds(beam):
+    """A product held to one pair of CTAs takes some 3 s and leaves the other SMs to the calls behind it, whose CTAs wait there.  What
+    they wait for that long is not a fault: bounded waits (2 s) begin when the call ahead has finished."""
+    n, k = 16384, 196608
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB")
+    a = torch.zeros(n, k, dtype=torch.float16, device="cuda")
+    a[:, 5] = 2
+    c = torch.empty(n, n, dtype=torch.float16, device="cuda")
+    x, w = normal((200, 256), torch.float16, 1), normal((64, 256), torch.float16, 2, 1 / 16)
+    xs, ws = normal((40, 4096), torch.float16, 3), normal((40, 4096), torch.float16, 4, 1 / 64)
+    shapes = [(200, 64), (3, 64), (200, 64), (200, 64), (200, 256), (40, 40)]
+    g = normal((200, 64), torch.float16, 6)
+    calls = [lambda o: beam.gated_gemmrc(x, w, w, o), lambda o: beam.gated_gemmrc(x[:3], w, w, o), lambda o: beam.gemmrc(x, w, o),
+             lambda o: beam.gemmrc(x, w, o, tile_n=128), lambda o: beam.gemmrc_backward(g, x, w, da=o),
+             lambda o: beam.cutlass_gemmrc_splitk(xs, ws, o, two_kernels=False)]
+    alone = [torch.zeros(s, dtype=torch.float16, device="cuda") for s in shapes]
+    behind = [torch.zeros_like(t) for t in alone]
+    for call, out in zip(calls, alone):
+        call(out)
+        torch.cuda.synchronize()
+    for first in (0, 1, 2, 5):
+        beam.gemmrc(a, a, c, max_ctas=2)
+        for j in range(6):
+            calls[(first + j) % 6](behind[(first + j) % 6])
+        torch.cuda.synchronize()
+        assert beam.device_status() == (0, 0)
+        assert (c == 4).all()
+        for out, want in zip(behind, alone):
+            assert torch.equal(out, want)
+            out.zero_()
 
 
 @pytest.mark.gpu
