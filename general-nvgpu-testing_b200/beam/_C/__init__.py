@@ -477,7 +477,8 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
 
         da = dg @ b_gate + du @ b_up,   db_gate = dg.T @ a,   db_up = du.T @ a.
 
-    dc, gate and up are [M,F]; gate and up are what the forward call kept.  The gradients wanted are given as tensors
+    dc, gate and up are [M,F]; gate and up are what the forward call kept (a gate of -inf, a product below the range of
+    float16, has the value and slope 0 that the product had).  The gradients wanted are given as tensors
     (at least one) and overwritten.  dg and du are rounded to the operands' type between the two steps; they are
     held in scratch of 4 M F bytes (and more for short batches) from torch's allocator."""
     act = _activation(activation)

@@ -234,7 +234,7 @@ BEAM_API int beam_gemmrc_silu(const void* A, const void* B, void* C, int m, int 
 
 /* ---- feed-forward block: gated product and gradients ---------------------------------------------- */
 
-/* Activations of the gated product, g the gate's projection: */
+/* Activations of the gated product, g the gate's projection (0 with slope 0 at g = -infinity, infinite with slope 1 at +infinity): */
 #define BEAM_ACT_SILU 0      /* g / (1 + exp(-g)) */
 #define BEAM_ACT_GELU 1      /* g (1 + erf(g / sqrt 2)) / 2 */
 #define BEAM_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
@@ -256,6 +256,7 @@ BEAM_API size_t beam_gated_gemmrc_backward_workspace_bytes(int m, int f, int k);
  *   dG = dC * up * act'(gate), dU = dC * act(gate)      (fp32, rounded once to the operands' type, in `workspace`: in fp16
  *                                                        they overflow above 65504, like any operand)
  *   dA = dG x B_gate + dU x B_up,  dB_gate = dG^T x A,  dB_up = dU^T x A      (fp32 accumulation, one rounding)
+ * A gate kept as -infinity, a product below the operands' range, has the value and slope 0 that the product had.
  * Any of dA, dB_gate and dB_up may be NULL, but not all three; B_gate and B_up may be NULL without dA, and A without dB_gate and
  * dB_up.  Outputs are overwritten (no accumulation into them), and overlap neither the inputs nor each other nor the workspace. */
 BEAM_API int beam_gated_gemmrc_backward(const void* dC, const void* A, const void* B_gate, const void* B_up,

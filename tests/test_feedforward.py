@@ -283,6 +283,39 @@ def test_activation_far_out(beam, healthy, act):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", (3, 200))
+def test_gradients_of_gates_past_the_range(beam, healthy, dtype, act, m):
+    """A gate's product far below what the type holds is kept as -infinity: act and its slope are 0 there, forward and backward, and
+    no gradient becomes NaN.  Above the range the slope is 1."""
+    f, k = 72, 136
+    a, bg, bu = gated_inputs(m, f, k, dtype, 17)
+    big = 1024.0 if dtype == torch.float16 else 2.0 ** 65
+    a[1, 3], bg[:, 3] = big, 0.0
+    bg[7, 3], bg[8, 3] = -big, big  # gates of row 1 near -big^2 and big^2
+    bu[:, 3] = 0.0
+    c, gate, up = (torch.empty(m, f, dtype=dtype, device="cuda") for _ in range(3))
+    beam.gated_gemmrc(a, bg, bu, c, activation=act, gate=gate, up=up)
+    assert torch.isneginf(gate[1, 7]) and torch.isposinf(gate[1, 8]) and gate.isinf().sum() == 2
+    assert c[1, 7] == 0 and torch.isinf(c[1, 8])
+    dc = normal((m, f), dtype, 18)
+    dbg, dbu, da = torch.empty_like(bg), torch.empty_like(bu), torch.empty_like(a)
+    # value and slope have their limits at -60000 and 60000 already, but for the value above
+    at = torch.where(gate.isinf(), gate.clamp(min=-60000, max=60000), gate)
+    v, slope = act64(act, at.double())
+    assert v[1, 7] == 0 and slope[1, 7] == 0 and slope[1, 8] == 1
+    beam.gated_gemmrc_backward(dc, a, bg, bu, gate, up, db_gate=dbg, activation=act)
+    check_gated_backward(dc, a, bg, bu, at, up, act, None, dbg, None)
+    dc[1, 8] = 0  # the value is infinite there, and so would be its gradients
+    gate[1, 8] = 1.0
+    at[1, 8] = 1.0
+    beam.gated_gemmrc_backward(dc, a, bg, bu, gate, up, da=da, db_gate=dbg, db_up=dbu, activation=act)
+    check_gated_backward(dc, a, bg, bu, at, up, act, da, dbg, dbu)
+    assert all(t.isfinite().all() for t in (da, dbg, dbu))
+
+
+@pytest.mark.gpu
 def test_gated_passes_nan_and_infinity_on(beam, healthy):
     """A NaN in one row of a reaches that row of c and no other; an infinite product stays infinite."""
     for m in (3, 200):
