@@ -74,6 +74,27 @@ void note_cuda_error(cudaError_t e, const char* where) {
 }
 const char* last_cuda_error_text() { return t_cuda_error; }
 
+namespace {
+
+// The fault word, zeroed.  The first call on a device may come while one of its streams is being captured into a graph (by this
+// thread, or by another one in the global mode): allocating is then only allowed in the relaxed mode, and the clearing must
+// stay off the legacy stream, which a capture of a blocking stream would involve.
+cudaError_t make_status_word(int** word) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return e;
+  cudaStream_t stream = nullptr;
+  e = cudaMalloc(word, 256);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(*word, 0, 256, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (stream) (void)cudaStreamDestroy(stream);
+  (void)cudaThreadExchangeStreamCaptureMode(&mode);
+  return e;
+}
+
+}  // namespace
+
 DeviceCtx* current_device_ctx(int* err) {
   int dev = -1;
   cudaError_t e = cudaGetDevice(&dev);
@@ -107,8 +128,7 @@ DeviceCtx* current_device_ctx(int* err) {
   c->cc_major = prop.major;
   c->cc_minor = prop.minor;
   c->cooperative_launch = prop.cooperativeLaunch != 0;
-  e = cudaMalloc(&c->status_word, 256);
-  if (e == cudaSuccess) e = cudaMemset(c->status_word, 0, 256);
+  e = make_status_word(&c->status_word);
   if (e != cudaSuccess) {
     note_cuda_error(e, "status word");
     (void)cudaGetLastError();
