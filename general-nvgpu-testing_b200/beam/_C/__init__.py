@@ -480,7 +480,7 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
     dc, gate and up are [M,F]; gate and up are what the forward call kept (a gate of -inf, a product below the range of
     float16, has the value and slope 0 that the product had).  The gradients wanted are given as tensors
     (at least one) and overwritten.  dg and du are rounded to the operands' type between the two steps; they are
-    held in scratch of 4 M F bytes (and more for short batches) from torch's allocator."""
+    held in scratch of 4 M F bytes (and more where there are few tiles and a long contraction) from torch's allocator."""
     act = _activation(activation)
     m, k = _check_first("a", a, _HALF_TYPES)
     dtype, dev, f = a.dtype, a.get_device(), _rows(b_gate)
@@ -505,8 +505,9 @@ def gated_gemmrc_backward(dc, a, b_gate, b_up, gate, up, da=None, db_gate=None, 
 
 
 def gemmrc_backward(dc, a, b, da=None, db=None):
-    """Gradients of c = a @ b.T: da[M,K] = dc[M,N] @ b[N,K] and db[N,K] = dc.T @ a[M,K], in one launch.  All tensors
-    float16 or all bfloat16; the gradients wanted are given (at least one) and overwritten; N and K multiples of 8."""
+    """Gradients of c = a @ b.T: da[M,K] = dc[M,N] @ b[N,K] and db[N,K] = dc.T @ a[M,K].  All tensors
+    float16 or all bfloat16; the gradients wanted are given (at least one) and overwritten; N and K multiples of 8.
+    Where there are few tiles and a long contraction, its sums go through scratch from torch's allocator."""
     m, k = _check_first("a", a, _HALF_TYPES)
     dtype, dev, n = a.dtype, a.get_device(), _rows(b)
     _check_matrix("b", b, (n, k), dtype, dev)

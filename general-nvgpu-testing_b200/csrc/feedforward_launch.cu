@@ -17,16 +17,18 @@ struct GatedPlan {
 
 // Up to 128 rows one CTA's tile holds them all and the weights are read once whatever the width, so the width only deals out F:
 // the smallest multiple of 8 with which the columns take as few waves of all SMs as 128-wide tiles would.  While that
-// leaves a CTA more k-blocks than bytes (a k-block takes its issuers about 0.14 us, in which an SM can read a width of 28),
-// clusters of 2 or 4 CTAs share a tile's contraction: wider tiles over fewer k-blocks, for an exchange of sums at the end.  Measured,
-// one row, us with 1 / 2 / 4 CTAs: F = 512, K = 4096 11.2 / 9.0 / 8.5; 2048, 4096 12.0 / 10.9 / 12.1; 4096, 4096 14.9 / 15.7 / 17.2;
+// leaves a CTA more k-blocks than bytes (a k-block takes its issuers about 0.14 us, in which an SM's share of the measured
+// bandwidth is a width of 24), clusters of 2 or 4 CTAs share a tile's contraction: wider tiles over fewer k-blocks, for an exchange
+// of sums at the end.  Measured, one row, us with 1 / 2 / 4 CTAs: F = 512, K = 4096 11.2 / 9.0 / 8.5; 2048, 4096 12.0 / 10.9 / 12.1; 4096, 4096 14.9 / 15.7 / 17.2;
 // 1024, 8192 18.6 / 13.3 / 12.2; 1024, 2048 7.7 / 7.3 / 7.7; 512, 1024 6.0 / 6.4 / 7.2.
 //
 // Above, pairs work on 256 rows.  A wave of narrower tiles is shorter, but not in proportion (A is read as often, and a UMMA
 // of N <= 128 is bound by its issue); measured per wave at K = 4096, in percent of a wave of 128-wide tiles: 96 columns 73 alone
 // and 78 among many waves, 64 columns 60, 32 columns 55.  The width with the least total is taken, the wider of two
 // that are equal: 128 for all large problems (4096 x 16384 x 4096: 681 us against 697 with 96 and 823 with 64), the narrowest
-// that still takes one wave for small ones (256 x 2048 x 2048: 11.1 us with 32 against 16.2 with 128).
+// that still takes one wave for small ones (256 x 2048 x 2048: 11.1 us with 32 against 16.2 with 128).  Pairs do not share a
+// contraction, so narrow layers with a long K take a step at 129 rows: 128 / 129 / 256 rows x 512 x 8192 11.4 / 16.8 / 16.9 us,
+// 1024 x 8192 12.9 / 17.2 / 17.3, 2048 x 8192 18.6 / 21.9 / 23.6, 2048 x 4096 12.0 / 11.8 / 12.2.
 GatedPlan gated_plan(int m, int f, int k, const int (&fit)[4]) {
   GatedPlan plan;
   if (m <= 128) {
@@ -306,7 +308,7 @@ int launch_grad(DeviceCtx* ctx, JobSpec* jobs, int n, int pairs, uint8_t* scratc
   p.group_m = 8;
   p.status = ctx->status_word;
   // Launches of whole waves, each at least kLaunchKBlocks k-blocks per pair (see grad_umma.cuh); a small list is one launch.
-  constexpr int kLaunchKBlocks = 1024;  // 0.28 ms
+  constexpr int kLaunchKBlocks = 1024;  // 0.33 ms at full clocks
   const int items = p.end;
   int st = BEAM_OK;
   for (p.begin = 0; p.begin < items && st == BEAM_OK; p.begin = p.end) {

@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(GatedShape<kCta>::kThreads, 1)
     __syncwarp();
     if constexpr (kCta == 1) {
       // The weights' first k-blocks may come into L2 while the kernel before this one finishes: a prefetch reads nothing, so
-      // it does not matter whether that kernel still writes them.  16 x 8192 x 4096: 25.7 -> 24.9 us; not worth its
+      // it does not matter whether that kernel still writes them.  16 x 8192 x 4096: 26.5 -> 25.9 us; not worth its
       // issue for narrow tiles (4 x 1024 x 2048: 7.3 -> 7.5).
       if (p.width > 32 && ptx::elect_one()) {
         for (int kb = 0; kb < min(num_kb, p.stages); ++kb) {  // one row of tiles: tile = column tile

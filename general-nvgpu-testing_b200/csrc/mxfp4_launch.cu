@@ -36,6 +36,9 @@ MxUnits lay_units(int rows, int k, int* grid) {
 // Where SMs are left over and K is long, clusters of 2 or 4 CTAs share a tile's contraction.  Measured, one row, us with
 // 1 / 2 / 4 CTAs: N = 2072, K = 8192 9.2 / 7.3 / 7.2; 1024, 4096 6.1 / 5.9 / 6.1; 4096, 4096 6.4 / 6.1; 2048, 2048 5.0 / 5.2 / 5.8; and
 // with 128 columns 9.9 / 8.1 / 7.3, 6.9 / 6.5 / 6.3, 7.3 / 6.7, 5.6 / 5.6 / 5.9.
+// Above 128 rows there is one form, 256 x 256 tiles on pairs over the whole of K.  It takes a step at 129 rows, since a few tiles
+// leave most pairs without work: 128 / 129 / 256 rows x 2048 x 8192 7.2 / 14.5 / 14.5 us, 4096 x 4096 6.6 / 10.2 / 10.2,
+// 4096 x 8192 8.7 / 14.9 / 15.1.
 struct NarrowPlan {
   int width, split;
 };

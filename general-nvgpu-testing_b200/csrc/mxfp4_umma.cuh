@@ -157,10 +157,9 @@ static __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint
 //              Two accumulators of 256 columns and the scales do not fit into 512 columns, so the accumulators overlap
 //              by 64 columns: the epilogue of a tile drains that part first and hands it back, after which the next
 //              tile's UMMAs may start in the other accumulator while the rest is drained.
-//              What bounds it at 8192^3 (177 us, 6.2 PFLOP/s): the tensor pipe is active 69 % of the cycles; copies alone
-//              (no UMMA, no scales) take 150 us, UMMAs without the scale copies 6 % less than with them, and each tile
-//              begins with a wait for the hand-back of about 1 us.  A sixth stage in place of the second store buffer
-//              took 190 us to 184; scales copied one stage ahead changed nothing (221 against 220).
+//              What bounds it at 8192^3 (182 us, 6.0 PFLOP/s): the tensor pipe is active 81 % of the cycles; the rest is the
+//              hand-back of the shared columns, some 2000 cycles for each of a pair's 14 tiles, and waits for operands.  A sixth
+//              stage is worth more than a second store buffer (3 % at this size).
 //   kCta = 1   M <= 128, bound by reading B: 128 rows x 64 or 128 columns (see narrow_plan() in mxfp4_launch.cu).  Only existing
 //              rows of A are loaded, two issuers take turns at the stages, and clusters may share a contraction, all
 //              as in gated_umma.cuh.
@@ -332,7 +331,7 @@ __global__ void __launch_bounds__(MxShape<kCta>::kThreads, 1) mxfp4_umma_kernel(
     __syncwarp();
     if constexpr (kCta == 1) {
       // B's first stages may come into L2 while the kernel before this one finishes (see gated_umma.cuh).  Wide tiles only:
-      // 1 x 16384 x 8192 with its quantisation 17.6 -> 16.9 us, but 16 x 8192 x 8192 (64-wide tiles) 13.0 -> 13.7.
+      // it takes 1 x 16384 x 8192 with its quantisation from 18.1 to 17.4 us, but adds 0.7 us to 16 x 8192 x 8192 (64-wide tiles).
       if (p.width > 64 && ptx::elect_one()) {
         for (int kb = 0; kb < min(num_kb, p.stages); ++kb)
           ptx::tma_prefetch_2d(&p.tm_b, (kb_base + kb) * 128, first * p.width);

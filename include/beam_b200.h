@@ -244,7 +244,7 @@ BEAM_API int beam_gemmrc_silu(const void* A, const void* B, void* C, int m, int 
  * product in one kernel (no counterpart in the reference).  A [M,K], B_gate and B_up [F,K], all fp16, or all bf16 with
  * BEAM_FLAG_BF16 (the only flag).  fp32 accumulation; G and U are combined in fp32 and C is rounded once.
  * gate, up: both NULL, or both [M,F] outputs that keep G and U (each rounded once) for the backward pass.
- * K % 8 == 0, F % 8 == 0, any M; outputs overlap neither the inputs nor each other. */
+ * K % 8 == 0, F % 8 == 0, any M >= 1; outputs overlap neither the inputs nor each other. */
 BEAM_API int beam_gated_gemmrc(const void* A, const void* B_gate, const void* B_up, void* C, void* gate, void* up, int m,
                                int f, int k, int activation, int flags, void* stream);
 
@@ -264,8 +264,8 @@ BEAM_API int beam_gated_gemmrc_backward(const void* dC, const void* A, const voi
                                         int f, int k, int activation, int flags, void* workspace,
                                         size_t workspace_bytes, void* stream);
 
-/* Gradients of the rc GEMM C = A x B^T: dA[M,K] = dC[M,N] x B[N,K] and dB[N,K] = dC^T x A[M,K], in one launch, without
- * transposing anything in memory.  fp16, or bf16 with BEAM_FLAG_BF16.  dA or dB may be NULL (then B, or A, may be too).
+/* Gradients of the rc GEMM C = A x B^T: dA[M,K] = dC[M,N] x B[N,K] and dB[N,K] = dC^T x A[M,K], as one list of tiles, without
+ * transposing anything in memory (a long list goes out in several launches).  fp16, or bf16 with BEAM_FLAG_BF16.  dA or dB may be NULL (then B, or A, may be too).
  * Where there are few tiles, a long contraction is cut into slices whose fp32 sums go through `workspace` and are added in a fixed
  * order by a second launch; beam_gemmrc_backward_workspace_bytes says how much that takes on the current device (0 for
  * most sizes; workspace may then be NULL). */
