@@ -179,3 +179,26 @@ def test_every_kind_of_call_on_three_streams(beam, healthy):
     for out in outs:
         for o, want in zip(out, alone):
             assert torch.equal(o, want)
+
+
+@pytest.mark.gpu
+def test_no_rows_are_refused(beam):
+    """An empty batch is an error that the host raises; nothing is launched and nothing written."""
+    a, bg, bu = gated_inputs(4, 16, 32, torch.float16)
+    c, none = torch.full((4, 16), 3.0, dtype=torch.float16, device="cuda"), torch.empty(0, 16, dtype=torch.float16, device="cuda")
+    db = torch.full_like(bg, 3.0)
+    with pytest.raises(ValueError):
+        beam.gated_gemmrc(a[:0], bg, bu, none)
+    with pytest.raises(ValueError):
+        beam.gated_gemmrc(a, bg[:0], bu[:0], c[:, :0].contiguous())
+    with pytest.raises(ValueError):
+        beam.gated_gemmrc_backward(none, a[:0], bg, bu, none, none, db_gate=db)
+    with pytest.raises(ValueError):
+        beam.gemmrc_backward(none, a[:0], bg, db=db)
+    q, scales = beam.mxfp4_empty(4, 32)
+    with pytest.raises(ValueError):
+        beam.mxfp4_quantize(a[:0], q[:0], scales[:0])
+    with pytest.raises(ValueError):
+        beam.mxfp4_gemmrc(q[:0], scales[:0], q, scales, none[:, :4].contiguous())
+    torch.cuda.synchronize()
+    assert (db == 3).all() and (c == 3).all()
